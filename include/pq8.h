@@ -78,6 +78,11 @@ extern "C" {
 #define PQ8_FLAG_FP32_PRODUCTS 4 /* pq8_rel_attention, pq8_stem: cuBLAS products in FP32 instead of TF32 */
 #define PQ8_ATTN_FP32 PQ8_FLAG_FP32_PRODUCTS
 
+/* ---- element types (the 8-bit product's tokens and outputs, the group norm) ---- */
+#define PQ8_TYPE_F32 0
+#define PQ8_TYPE_F16 1
+#define PQ8_TYPE_BF16 2
+
 #define PQ8_HEADER_BYTES 256
 #define PQ8_TILE_ROWS 128
 #define PQ8_RECORD_BYTES 4352 /* 128 rows x 32 int8 + 128 fp16 scales */
@@ -469,6 +474,77 @@ PQ8_API int pq8_stem(const float* mel, int windows, int frames, const float* w0,
                      const float* b2, const float* w3, const float* b3, const float* w5, const float* b5,
                      const float* w6, const float* b6, const void* w_out, const float* b_out, float* out, int flags,
                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- products in 8-bit integers ----------------------------------------------
+ * The Q8_0 entry points above multiply in TF32. These multiply 8-bit integers
+ * with 32-bit integer sums (the sums are exact): weights with one scale per
+ * output channel, tokens with one scale per row, found on the way. They have
+ * no counterpart in the reference, whose products are FP32 (gpu.py:87-90).
+ *
+ * A row h of tokens becomes s = max|h| / 127 (rounded to FP32) and
+ * q = h / s rounded to the nearest integer, ties to even, in [-127, 127]; the
+ * integers are those of the exact quotient. A row of zeros has s = 0 and
+ * q = 0; a row that holds an infinity or a NaN has s = NaN and q = 0, so that
+ * its outputs are NaN and no other row's.
+ * Types are PQ8_TYPE_*; ld is the distance of two rows in elements (>= width).
+ * `width` / `k` is a positive multiple of 16, q 16-byte aligned and dense.
+ * x needs its type's alignment only; rows whose start and distance are
+ * multiples of 16 bytes are read fastest. */
+PQ8_API int pq8_quantize_rows(const void* x, int type, long long ld, int8_t* q, float* scale, int rows, int width,
+                              void* stream);
+
+/* LayerNorm (eps 1e-5, as pq8_layer_norm) and quantisation of its result in
+ * one pass: no normalised row is written. w, b: float[width]. Mean and
+ * variance are FP64. Values of 2^126 and beyond count as infinite. */
+PQ8_API int pq8_layer_norm_quantize(const void* x, int type, long long ld, const float* w, const float* b, int8_t* q,
+                                    float* scale, int rows, int width, void* stream);
+
+/* The product of quantised tokens x [m, k] with weights w [n, k] (both dense,
+ * 16-byte aligned): z[m, j] = x_scale[m] * w_scale[j] * sum_k x[m, k] w[j, k]
+ * (+ bias[j]), y = epilogue(z) rounded once to y_type. Epilogues as pq8_gemm;
+ * PQ8_EPI_GLU takes plain rows (y[:, j] = z[:, j] sigmoid(z[:, j + n / 2]), n
+ * even: no packed layout). bias: float[n] or NULL; resid: y's type and
+ * shape (EPI_RESIDUAL only), may be y itself. y may overlap none of the other inputs.
+ * k at most 131,056, so that no sum leaves 32 bits. Any m >= 0, n >= 1. */
+PQ8_API int pq8_gemm_i8(const int8_t* w, const float* w_scale, const int8_t* x, const float* x_scale, void* y,
+                        int y_type, const float* bias, const void* resid, int m, int n, int k, int epilogue,
+                        float alpha, void* stream);
+
+/* pq8_quantize_rows (norm_w, norm_b NULL) or pq8_layer_norm_quantize, then
+ * pq8_gemm_i8: the linear on tokens in floating point. The
+ * quantised tokens live in the workspace (16-byte aligned, no
+ * initialisation): calls that may overlap on the GPU need one each. */
+PQ8_API int pq8_linear_i8_workspace_size(int m, int k, size_t* bytes);
+PQ8_API int pq8_linear_i8(const int8_t* w, const float* w_scale, const void* x, int x_type, long long ld,
+                          const float* norm_w, const float* norm_b, void* y, int y_type, const float* bias,
+                          const void* resid, int m, int n, int k, int epilogue, float alpha, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* ---- group norm ----------------------------------------------------------------
+ * Group norm with an activation, channels last, for conv modules that use it in
+ * BatchNorm's place: x, y [rows][channels] (dense, of `type`); windows of
+ * consecutive rows; mean and variance over the rows of one window and the
+ * channels / groups channels of one group, y = act((x - mean) / sqrt(var +
+ * eps) * w + b) with act PQ8_EPI_NONE, PQ8_EPI_RELU or PQ8_EPI_SILU. w, b:
+ * float[channels]. offsets: device int[windows + 1], window i has rows
+ * offsets[i] to offsets[i + 1] - 1 (windows of no rows are fine; they should
+ * not overlap: a row in two windows gets the values of either; an offset
+ * outside 0..rows is held to that range, and a window that ends before it
+ * starts is empty), rows of y in no window are not written; or NULL: windows of rows / windows rows each.
+ * Sums are FP64, in a fixed order. channels at most 16384, groups at most
+ * 4096, rows at most 2^30. y must not overlap x. PQ8_FLAG_OUT_TF32 (type F32)
+ * rounds y for a following pq8_gemm. The workspace (16-byte aligned, no
+ * initialisation) is per call in flight. No counterpart in the reference,
+ * whose conv module has BatchNorm (reference.py:60-63). */
+PQ8_API int pq8_group_norm_workspace_size(int rows, int windows, int channels, int groups, size_t* bytes);
+PQ8_API int pq8_group_norm(const void* x, int type, const float* w, const float* b, void* y, int rows, int windows,
+                           const int* offsets, int channels, int groups, double eps, int activation, int flags,
+                           void* workspace, size_t workspace_bytes, void* stream);
+/* The same, its rows quantised as pq8_quantize_rows quantises them (channels
+ * a multiple of 16): q [rows][channels], scale [rows], for pq8_gemm_i8. */
+PQ8_API int pq8_group_norm_quantize(const void* x, int type, const float* w, const float* b, int8_t* q, float* scale,
+                                    int rows, int windows, const int* offsets, int channels, int groups, double eps,
+                                    int activation, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

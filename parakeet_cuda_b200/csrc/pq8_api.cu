@@ -19,6 +19,9 @@
 #include "pq8_tdt.cuh"
 #include "pq8_decode.cuh"
 #include "pq8_attention.cuh"
+#include "pq8_rows.cuh"
+#include "pq8_i8.cuh"
+#include "pq8_group_norm.cuh"
 
 namespace pq8 {
 
@@ -2080,4 +2083,387 @@ extern "C" int pq8_stem(const float* mel, int windows, int frames, const float* 
   // the output linear, Q8_0 [1024, 4096] + bias, on the TF32-rounded flattened rows
   return pq8_gemm(w_out, flat, out, b_out, nullptr, static_cast<int>(rows), 1024, 4096, PQ8_EPI_NONE, 1.0f,
                   PQ8_FLAG_X_TF32, stream);
+}
+
+// ---------------------------------------------------------------- 8-bit products
+namespace pq8 {
+namespace {
+
+constexpr double kNormEps64 = 1e-5;  // reference.py:8
+constexpr int kI8MaxK = 131056;      // 128 * 128 * k stays below 2^31
+
+int type_size(int type) { return type == PQ8_TYPE_F32 ? 4 : type == PQ8_TYPE_F16 || type == PQ8_TYPE_BF16 ? 2 : 0; }
+
+// f(a value of the element type)
+template <typename F>
+auto with_type(int type, F&& f) {
+  return type == PQ8_TYPE_F32 ? f(float{}) : type == PQ8_TYPE_F16 ? f(__half{}) : f(__nv_bfloat16{});
+}
+
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a != nullptr && b != nullptr && x < y + nb && y < x + na;
+}
+// y may be resid itself, and overlaps nothing that is read otherwise.
+bool resid_ok(const void* y, const void* resid, size_t bytes) {
+  return y == resid || !overlap(y, bytes, resid, bytes);
+}
+
+size_t rows_bytes(long long rows, long long ld, int width, int size) {
+  return static_cast<size_t>((rows - 1) * ld + width) * size;
+}
+
+int check_rows_args(const void* x, int type, long long ld, const float* w, const float* b, const int8_t* q,
+                    const float* scale, int rows, int width) {
+  if (rows < 0 || width <= 0 || width % 16 || width > kI8MaxK) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  const int size = type_size(type);
+  if (size == 0 || (w == nullptr) != (b == nullptr)) return PQ8_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return PQ8_OK;
+  if (x == nullptr || q == nullptr || scale == nullptr || ld < width) return PQ8_ERR_INVALID_ARGUMENT;
+  if (ld > (1LL << 40)) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  if (!aligned(x, size) || !aligned(q, 16) || !aligned(scale, 4) || !aligned(w, 4) || !aligned(b, 4))
+    return PQ8_ERR_MISALIGNED;
+  const size_t nx = rows_bytes(rows, ld, width, size);
+  if (overlap(x, nx, q, static_cast<size_t>(rows) * width) || overlap(x, nx, scale, static_cast<size_t>(rows) * 4))
+    return PQ8_ERR_INVALID_ARGUMENT;
+  return PQ8_OK;
+}
+
+template <typename T, int CHUNKS, int WARPS>
+cudaError_t launch_rows(DeviceState* ds, const T* x, long long ld, const float* w, const float* b, int8_t* q,
+                        float* scale, int rows, int width, cudaStream_t st) {
+  constexpr int kTeams = kRowThreads / (32 * WARPS);
+  const int vec = aligned(x, 16) && (ld * sizeof(T)) % 16 == 0;
+  const dim3 grid(static_cast<unsigned>(std::min<long long>((rows + kTeams - 1LL) / kTeams, 8LL * ds->sms)));
+  if (w != nullptr)
+    return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, true>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
+                      kNormEps64, q, scale, rows, width, vec);
+  return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, false>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
+                    kNormEps64, q, scale, rows, width, vec);
+}
+
+// A warp per row while 32 lanes x 32 values hold it, then a CTA per row while
+// 256 x 32 do, then rows read again in each pass.
+template <typename T>
+cudaError_t launch_rows_typed(DeviceState* ds, const T* x, long long ld, const float* w, const float* b, int8_t* q,
+                              float* scale, int rows, int width, cudaStream_t st) {
+  constexpr int C = 32 / kChunk<T>;
+  if (width <= 1024) return launch_rows<T, C, 1>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (width <= 8192) return launch_rows<T, C, 8>(ds, x, ld, w, b, q, scale, rows, width, st);
+  return launch_rows<T, 0, 8>(ds, x, ld, w, b, q, scale, rows, width, st);
+}
+
+int quantize_rows(const void* x, int type, long long ld, const float* w, const float* b, int8_t* q, float* scale,
+                  int rows, int width, void* stream) {
+  int rc = check_rows_args(x, type, ld, w, b, q, scale, rows, width);
+  if (rc || rows == 0) return rc;
+  DeviceState* ds;
+  if ((rc = device_state(&ds))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = with_type(type, [&](auto t) {
+    using T = decltype(t);
+    return launch_rows_typed<T>(ds, static_cast<const T*>(x), ld, w, b, q, scale, rows, width, st);
+  });
+  if (e != cudaSuccess) return to_code(e);
+  return to_code(cudaGetLastError());
+}
+
+int check_i8_args(const int8_t* w, const float* w_scale, const void* y, int y_type, const void* resid, int m, int n,
+                  int k, int epilogue) {
+  if (m < 0 || n < 1 || k <= 0 || k % 16 || k > kI8MaxK) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  if (epilogue < PQ8_EPI_NONE || epilogue > PQ8_EPI_RESIDUAL || type_size(y_type) == 0)
+    return PQ8_ERR_INVALID_ARGUMENT;
+  if (epilogue == PQ8_EPI_GLU && n % 2) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  if (m == 0) return PQ8_OK;
+  if (w == nullptr || w_scale == nullptr || y == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  if (epilogue == PQ8_EPI_RESIDUAL && resid == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  if (!aligned(w, 16) || !aligned(w_scale, 4) || !aligned(y, type_size(y_type)) ||
+      !aligned(resid, type_size(y_type)))
+    return PQ8_ERR_MISALIGNED;
+  return PQ8_OK;
+}
+
+template <typename T, int M>
+cudaError_t launch_i8_gemv(const I8Params& p, int sms, cudaStream_t st) {
+  const int warps = kI8GemvThreads / 32;
+  const bool glu = p.epi == PQ8_EPI_GLU;
+  auto go = [&](auto kernel, int per_warp) {
+    const dim3 grid((p.out_cols + per_warp * warps - 1) / (per_warp * warps), std::min((p.m + M - 1) / M, 32768));
+    return launch_pdl(kernel, grid, dim3(kI8GemvThreads), 0, st, p);
+  };
+  if (p.n >= 4 * warps * sms) return go(i8_gemv_kernel<T, M, 4>, glu ? 2 : 4);
+  if (p.n >= 2 * warps * sms || glu) return go(i8_gemv_kernel<T, M, 2>, glu ? 1 : 2);
+  return go(i8_gemv_kernel<T, M, 1>, 1);
+}
+
+int launch_i8(DeviceState* ds, const I8Params& p, int y_type, cudaStream_t st) {
+  const cudaError_t e = with_type(y_type, [&](auto t) {
+    using T = decltype(t);
+    return p.m <= 1   ? launch_i8_gemv<T, 1>(p, ds->sms, st)
+           : p.m <= 2 ? launch_i8_gemv<T, 2>(p, ds->sms, st)
+           : p.m <= 4 ? launch_i8_gemv<T, 4>(p, ds->sms, st)
+                      : launch_i8_gemv<T, 8>(p, ds->sms, st);
+  });
+  if (e != cudaSuccess) return to_code(e);
+  return to_code(cudaGetLastError());
+}
+
+I8Params i8_params(DeviceState* ds, const int8_t* w, const float* w_scale, const int8_t* x, const float* x_scale,
+                   void* y, const float* bias, const void* resid, int m, int n, int k, int epilogue, float alpha) {
+  I8Params p{};
+  p.w = w;
+  p.w_scale = w_scale;
+  p.x = x;
+  p.x_scale = x_scale;
+  p.y = y;
+  p.bias = bias;
+  p.resid = epilogue == PQ8_EPI_RESIDUAL ? resid : nullptr;
+  p.status = ds->status;
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.epi = epilogue;
+  p.out_cols = epilogue == PQ8_EPI_GLU ? n / 2 : n;
+  p.alpha = alpha;
+  return p;
+}
+
+// Nothing that is read overlaps y (the residual may be y itself).
+int check_i8_overlap(const int8_t* w, const float* w_scale, const void* x, size_t x_bytes, const float* x_scale,
+                     const void* y, int y_type, const float* bias, const void* resid, int m, int n, int k,
+                     int epilogue) {
+  const size_t ny = static_cast<size_t>(m) * (epilogue == PQ8_EPI_GLU ? n / 2 : n) * type_size(y_type);
+  if (overlap(y, ny, w, static_cast<size_t>(n) * k) || overlap(y, ny, w_scale, static_cast<size_t>(n) * 4) ||
+      overlap(y, ny, x, x_bytes) || overlap(y, ny, x_scale, static_cast<size_t>(m) * 4) ||
+      overlap(y, ny, bias, static_cast<size_t>(n) * 4) ||
+      (epilogue == PQ8_EPI_RESIDUAL && !resid_ok(y, resid, ny)))
+    return PQ8_ERR_INVALID_ARGUMENT;
+  return PQ8_OK;
+}
+
+struct I8Workspace {
+  size_t scale, total;  // q at 0
+};
+I8Workspace plan_linear_i8(int m, int k) {
+  I8Workspace w;
+  w.scale = round256(static_cast<size_t>(m) * k);
+  w.total = w.scale + round256(static_cast<size_t>(m) * 4);
+  return w;
+}
+
+}  // namespace
+}  // namespace pq8
+
+extern "C" int pq8_quantize_rows(const void* x, int type, long long ld, int8_t* q, float* scale, int rows, int width,
+                                 void* stream) {
+  return quantize_rows(x, type, ld, nullptr, nullptr, q, scale, rows, width, stream);
+}
+
+extern "C" int pq8_layer_norm_quantize(const void* x, int type, long long ld, const float* w, const float* b,
+                                       int8_t* q, float* scale, int rows, int width, void* stream) {
+  if (rows > 0 && (w == nullptr || b == nullptr)) return PQ8_ERR_INVALID_ARGUMENT;
+  return quantize_rows(x, type, ld, w, b, q, scale, rows, width, stream);
+}
+
+extern "C" int pq8_gemm_i8(const int8_t* w, const float* w_scale, const int8_t* x, const float* x_scale, void* y,
+                           int y_type, const float* bias, const void* resid, int m, int n, int k, int epilogue,
+                           float alpha, void* stream) {
+  int rc = check_i8_args(w, w_scale, y, y_type, resid, m, n, k, epilogue);
+  if (rc || m == 0) return rc;
+  if (x == nullptr || x_scale == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  if (!aligned(x, 16) || !aligned(x_scale, 4) || !aligned(bias, 4)) return PQ8_ERR_MISALIGNED;
+  if ((rc = check_i8_overlap(w, w_scale, x, static_cast<size_t>(m) * k, x_scale, y, y_type, bias, resid, m, n, k,
+                             epilogue)))
+    return rc;
+  DeviceState* ds;
+  if ((rc = device_state(&ds))) return rc;
+  return launch_i8(ds, i8_params(ds, w, w_scale, x, x_scale, y, bias, resid, m, n, k, epilogue, alpha), y_type,
+                   static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int pq8_linear_i8_workspace_size(int m, int k, size_t* bytes) {
+  if (bytes == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  if (m < 0 || k <= 0 || k % 16 || k > kI8MaxK) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  *bytes = plan_linear_i8(m, k).total;
+  return PQ8_OK;
+}
+
+extern "C" int pq8_linear_i8(const int8_t* w, const float* w_scale, const void* x, int x_type, long long ld,
+                             const float* norm_w, const float* norm_b, void* y, int y_type, const float* bias,
+                             const void* resid, int m, int n, int k, int epilogue, float alpha, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  int rc = check_i8_args(w, w_scale, y, y_type, resid, m, n, k, epilogue);
+  if (rc) return rc;
+  const I8Workspace ws = plan_linear_i8(m, k);
+  if (m > 0 && (workspace == nullptr || workspace_bytes < ws.total)) return PQ8_ERR_WORKSPACE;
+  if (!aligned(workspace, 16) || !aligned(bias, 4)) return PQ8_ERR_MISALIGNED;
+  int8_t* q = static_cast<int8_t*>(workspace);
+  float* scale = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + ws.scale);
+  if ((rc = check_rows_args(x, x_type, ld, norm_w, norm_b, q, scale, m, k)) || m == 0) return rc;
+  if ((rc = check_i8_overlap(w, w_scale, x, rows_bytes(m, ld, k, type_size(x_type)), scale, y, y_type, bias, resid, m,
+                             n, k, epilogue)))
+    return rc;
+  DeviceState* ds;
+  if ((rc = device_state(&ds))) return rc;
+  if ((rc = quantize_rows(x, x_type, ld, norm_w, norm_b, q, scale, m, k, stream))) return rc;
+  return launch_i8(ds, i8_params(ds, w, w_scale, q, scale, y, bias, resid, m, n, k, epilogue, alpha), y_type,
+                   static_cast<cudaStream_t>(stream));
+}
+
+// ---------------------------------------------------------------- group norm
+namespace pq8 {
+namespace {
+
+struct GroupNormPlan {
+  int chunks, slab, slabs, grid_y;
+  size_t total;
+};
+
+// Row chunks per window so that windows x slabs x chunks fill the SMs a few
+// times, with at least 8 rows a chunk.
+GroupNormPlan plan_group_norm(int rows, int windows, int channels, int groups) {
+  GroupNormPlan g{};
+  const int cg = channels / groups;
+  g.slab = std::max(1, std::min(groups, kNormThreads / cg));
+  g.slabs = (groups + g.slab - 1) / g.slab;
+  const int per_window = std::max(1, rows / std::max(1, windows));
+  const long long units = static_cast<long long>(windows) * g.slabs;
+  g.chunks = static_cast<int>(std::max<long long>(1, std::min<long long>({64, (per_window + 7) / 8, 1184 / units})));
+  g.grid_y = std::min(windows, 65535);
+  g.total = round256(sizeof(GroupSum) * static_cast<size_t>(windows) * g.chunks * groups);
+  return g;
+}
+
+int check_group_norm(const void* x, int type, const float* w, const float* b, const void* y, size_t y_bytes, int rows,
+                     int windows, const int* offsets, int channels, int groups, double eps, int act, void* workspace,
+                     size_t workspace_bytes) {
+  if (rows < 0 || rows > (1 << 30) || windows < 0 || windows > (1 << 24) || channels < 1 || channels > 16384 ||
+      groups < 1 || groups > 4096 || channels % groups)
+    return PQ8_ERR_UNSUPPORTED_SHAPE;
+  if (offsets == nullptr && windows > 0 && rows % windows) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  const int size = type_size(type);
+  if (size == 0 || !(eps > 0.0) || !(eps < 1e30) ||
+      (act != PQ8_EPI_NONE && act != PQ8_EPI_RELU && act != PQ8_EPI_SILU))
+    return PQ8_ERR_INVALID_ARGUMENT;
+  if (rows == 0 || windows == 0) return PQ8_OK;
+  if (x == nullptr || w == nullptr || b == nullptr || y == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  if (!aligned(x, size) || !aligned(w, 4) || !aligned(b, 4) || !aligned(offsets, 4) || !aligned(workspace, 16))
+    return PQ8_ERR_MISALIGNED;
+  if (overlap(y, y_bytes, x, static_cast<size_t>(rows) * channels * size) ||
+      overlap(y, y_bytes, w, static_cast<size_t>(channels) * 4) ||
+      overlap(y, y_bytes, b, static_cast<size_t>(channels) * 4) ||
+      overlap(y, y_bytes, offsets, (static_cast<size_t>(windows) + 1) * 4))
+    return PQ8_ERR_INVALID_ARGUMENT;
+  const GroupNormPlan g = plan_group_norm(rows, windows, channels, groups);
+  if (workspace == nullptr || workspace_bytes < g.total) return PQ8_ERR_WORKSPACE;
+  return PQ8_OK;
+}
+
+GroupNormParams group_norm_params(const GroupNormPlan& g, const void* x, const float* w, const float* b, int rows,
+                                  int windows, const int* offsets, int channels, int groups, double eps, int act) {
+  GroupNormParams p{};
+  p.x = x;
+  p.w = w;
+  p.b = b;
+  p.offsets = offsets;
+  p.rows = rows;
+  p.windows = windows;
+  p.channels = channels;
+  p.groups = groups;
+  p.epi = act;
+  p.eps = eps;
+  p.chunks = g.chunks;
+  p.slab = g.slab;
+  return p;
+}
+
+template <typename T>
+cudaError_t launch_group_stats(const GroupNormPlan& g, const GroupNormParams& p, bool vec, GroupSum* partial,
+                               cudaStream_t st) {
+  const dim3 grid(g.chunks, g.grid_y, g.slabs);
+  return vec ? launch_pdl(group_stats_kernel<T, true>, grid, dim3(kNormThreads), 0, st, p, partial)
+             : launch_pdl(group_stats_kernel<T, false>, grid, dim3(kNormThreads), 0, st, p, partial);
+}
+
+}  // namespace
+}  // namespace pq8
+
+extern "C" int pq8_group_norm_workspace_size(int rows, int windows, int channels, int groups, size_t* bytes) {
+  if (bytes == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  if (rows < 0 || rows > (1 << 30) || windows < 0 || windows > (1 << 24) || channels < 1 || channels > 16384 ||
+      groups < 1 || groups > 4096 || channels % groups)
+    return PQ8_ERR_UNSUPPORTED_SHAPE;
+  *bytes = plan_group_norm(rows, windows, channels, groups).total;
+  return PQ8_OK;
+}
+
+extern "C" int pq8_group_norm(const void* x, int type, const float* w, const float* b, void* y, int rows, int windows,
+                              const int* offsets, int channels, int groups, double eps, int activation, int flags,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  if (type_size(type) == 0 || (flags & ~PQ8_FLAG_OUT_TF32) || ((flags & PQ8_FLAG_OUT_TF32) && type != PQ8_TYPE_F32))
+    return PQ8_ERR_INVALID_ARGUMENT;
+  const size_t bytes = static_cast<size_t>(std::max(rows, 0)) * std::max(channels, 0) * type_size(type);
+  int rc = check_group_norm(x, type, w, b, y, bytes, rows, windows, offsets, channels, groups, eps, activation,
+                            workspace, workspace_bytes);
+  if (rc || rows == 0 || windows == 0) return rc;
+  if (!aligned(y, type_size(type))) return PQ8_ERR_MISALIGNED;
+  DeviceState* ds;
+  if ((rc = device_state(&ds))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const GroupNormPlan g = plan_group_norm(rows, windows, channels, groups);
+  const cudaError_t e = with_type(type, [&](auto t) {
+    using T = decltype(t);
+    GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
+    p.round_out = (flags & PQ8_FLAG_OUT_TF32) ? 1 : 0;
+    const bool vec = (channels / groups) % kChunk<T> == 0 && aligned(x, 16) && aligned(y, 16);
+    GroupSum* partial = static_cast<GroupSum*>(workspace);
+    cudaError_t err = launch_group_stats<T>(g, p, vec, partial, st);
+    if (err != cudaSuccess) return err;
+    const dim3 grid(g.chunks, g.grid_y, g.slabs);
+    const size_t smem = sizeof(GroupStat) * g.slab;
+    return vec ? launch_pdl(group_apply_kernel<T, true>, grid, dim3(kNormThreads), smem, st, p,
+                            static_cast<const GroupSum*>(partial), static_cast<T*>(y))
+               : launch_pdl(group_apply_kernel<T, false>, grid, dim3(kNormThreads), smem, st, p,
+                            static_cast<const GroupSum*>(partial), static_cast<T*>(y));
+  });
+  if (e != cudaSuccess) return to_code(e);
+  return to_code(cudaGetLastError());
+}
+
+extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, const float* b, int8_t* q,
+                                       float* scale, int rows, int windows, const int* offsets, int channels,
+                                       int groups, double eps, int activation, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  if (channels % 16) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  const size_t bytes = static_cast<size_t>(std::max(rows, 0)) * std::max(channels, 0);
+  int rc = check_group_norm(x, type, w, b, q, bytes, rows, windows, offsets, channels, groups, eps, activation,
+                            workspace, workspace_bytes);
+  if (rc || rows == 0 || windows == 0) return rc;
+  if (scale == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  if (!aligned(q, 16) || !aligned(scale, 4)) return PQ8_ERR_MISALIGNED;
+  DeviceState* ds;
+  if ((rc = device_state(&ds))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const GroupNormPlan g = plan_group_norm(rows, windows, channels, groups);
+  const cudaError_t e = with_type(type, [&](auto t) {
+    using T = decltype(t);
+    GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
+    p.vec = aligned(x, 16);
+    GroupSum* partial = static_cast<GroupSum*>(workspace);
+    cudaError_t err = launch_group_stats<T>(g, p, p.vec && (channels / groups) % kChunk<T> == 0, partial, st);
+    if (err != cudaSuccess) return err;
+    const dim3 grid(g.chunks * g.slabs, g.grid_y);
+    const size_t smem = sizeof(GroupStat) * groups;
+    constexpr int C = 32 / kChunk<T>;
+    auto kernel = channels <= 1024   ? group_quantize_kernel<T, C, 1>
+                  : channels <= 8192 ? group_quantize_kernel<T, C, 8>
+                                     : group_quantize_kernel<T, 0, 8>;
+    if (smem > 48 * 1024 - 256) {
+      err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (err != cudaSuccess) return err;
+    }
+    return launch_pdl(kernel, grid, dim3(kRowThreads), smem, st, p, static_cast<const GroupSum*>(partial), q, scale);
+  });
+  if (e != cudaSuccess) return to_code(e);
+  return to_code(cudaGetLastError());
 }

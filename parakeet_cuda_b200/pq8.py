@@ -34,11 +34,13 @@ LAYOUT_ROWS, LAYOUT_GLU, LAYOUT_GATES4 = 0, 1, 2
 EPI_NONE, EPI_RELU, EPI_SILU, EPI_GLU, EPI_RESIDUAL = 0, 1, 2, 3, 4
 FLAG_X_TF32, FLAG_OUT_TF32, FLAG_FP32_PRODUCTS = 1, 2, 4
 ATTN_FP32 = FLAG_FP32_PRODUCTS
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+I8_MAX_K = 131056        # sums of k products of two 8-bit integers stay within 32 bits
 HEADER_BYTES, TILE_ROWS, RECORD_BYTES = 256, 128, 4352
 GEMV_MAX_M = 64          # rows the GEMV entry points take (row groups of 8 run in one launch)
 LINEAR_GEMV_MAX_M = 8    # pq8_linear's GEMV/GEMM dispatch threshold
 
-_P, _I, _F, _SZ, _LL = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_longlong
+_P, _I, _F, _D, _SZ, _LL = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_size_t, C.c_longlong
 
 
 class GemmTask(C.Structure):
@@ -98,6 +100,14 @@ SIGNATURES = {
     'pq8_tdt_decode_workspace_size': ([_I, _I, _I, C.POINTER(_SZ)], _I),
     'pq8_tdt_decode': ([C.POINTER(TdtWeights), _P, _I, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _P, _P, _P, _SZ,
                         _P], _I),
+    'pq8_quantize_rows': ([_P, _I, _LL, _P, _P, _I, _I, _P], _I),
+    'pq8_layer_norm_quantize': ([_P, _I, _LL, _P, _P, _P, _P, _I, _I, _P], _I),
+    'pq8_gemm_i8': ([_P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _P], _I),
+    'pq8_linear_i8_workspace_size': ([_I, _I, C.POINTER(_SZ)], _I),
+    'pq8_linear_i8': ([_P, _P, _P, _I, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _P, _SZ, _P], _I),
+    'pq8_group_norm_workspace_size': ([_I, _I, _I, _I, C.POINTER(_SZ)], _I),
+    'pq8_group_norm': ([_P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _D, _I, _I, _P, _SZ, _P], _I),
+    'pq8_group_norm_quantize': ([_P, _I, _P, _P, _P, _P, _I, _I, _P, _I, _I, _D, _I, _P, _SZ, _P], _I),
 }
 
 
@@ -167,6 +177,16 @@ class Library:
     def linear_workspace_size(self, m: int, n: int, k: int) -> int:
         out = _SZ()
         self.call('pq8_linear_workspace_size', m, n, k, C.byref(out))
+        return out.value
+
+    def linear_i8_workspace_size(self, m: int, k: int) -> int:
+        out = _SZ()
+        self.call('pq8_linear_i8_workspace_size', m, k, C.byref(out))
+        return out.value
+
+    def group_norm_workspace_size(self, rows: int, windows: int, channels: int, groups: int) -> int:
+        out = _SZ()
+        self.call('pq8_group_norm_workspace_size', rows, windows, channels, groups, C.byref(out))
         return out.value
 
     def stem_workspace_size(self, windows: int, frames: int) -> int:

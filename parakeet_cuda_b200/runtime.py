@@ -22,7 +22,8 @@ import numpy as np
 import torch
 
 from . import pq8
-from .pq8 import EPI_GLU, EPI_NONE, GEMV_MAX_M, LAYOUT_GATES4, LAYOUT_GLU, LAYOUT_ROWS
+from .pq8 import (EPI_GLU, EPI_NONE, GEMV_MAX_M, LAYOUT_GATES4, LAYOUT_GLU, LAYOUT_ROWS, TYPE_BF16,
+                  TYPE_F16, TYPE_F32)
 
 MIB = 1 << 20
 
@@ -46,6 +47,25 @@ class PackedWeight:
     @property
     def out_features(self) -> int:
         return self.n // 2 if self.layout == LAYOUT_GLU else self.n // 4 if self.layout == LAYOUT_GATES4 else self.n
+
+
+#: Element types of the 8-bit product's tokens and outputs and of the group norm.
+ELEMENT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+
+
+@dataclass
+class Int8Weight:
+    """Weights for the product in 8-bit integers: ``q`` int8 [n, k] (dense), ``scale`` float32 [n]."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+@dataclass
+class QuantizedRows:
+    """Tokens quantised row by row: ``q`` int8 [rows, width] (dense), ``scale`` float32 [rows];
+    row i stands for ``q[i] * scale[i]``."""
+    q: torch.Tensor
+    scale: torch.Tensor
 
 
 def pack_host(raw, n: int, k: int, layout: int = LAYOUT_ROWS, lib=None) -> np.ndarray:
@@ -268,6 +288,176 @@ class Runtime:
                               device=self.device)
         self.lib.call('pq8_gemm', w.pointer, x.data_ptr(), out.data_ptr(), _ptr(bias), _ptr(resid), rows, w.n, k,
                       epilogue, float(alpha), flags, self.stream())
+        return out
+
+    # -- products in 8-bit integers -------------------------------------------
+    def _check(self, t: torch.Tensor, what: str, dtype=None, shape=None) -> None:
+        """A dense tensor on this device, of ``dtype`` and ``shape`` where given."""
+        if t.device != self.device:
+            raise ValueError(f'{what} is on {t.device}, the runtime on {self.device}')
+        if dtype is not None and t.dtype != dtype:
+            raise ValueError(f'{what} must be {dtype}, got {t.dtype}')
+        if shape is not None and t.shape != shape:
+            raise ValueError(f'{what} must have shape {tuple(shape)}, got {tuple(t.shape)}')
+        if not t.is_contiguous():
+            raise ValueError(f'{what} must be contiguous')
+
+    def _check_rows(self, x: torch.Tensor) -> tuple[int, int, int, int]:
+        """(rows, width, row distance, type code) of a matrix whose rows are dense."""
+        kind = ELEMENT_TYPES.get(x.dtype)
+        if kind is None:
+            raise ValueError(f'x must be float32, float16 or bfloat16, got {x.dtype}')
+        if x.dim() != 2:
+            raise ValueError(f'x must be a matrix, got {x.dim()} dimensions')
+        if x.device != self.device:
+            raise ValueError(f'x is on {x.device}, the runtime on {self.device}')
+        rows, width = x.shape
+        ld, step = x.stride()
+        if rows <= 1:
+            ld = width
+        if step != 1 and width > 1 or ld < width:
+            raise ValueError(f'the rows of x must be dense and apart, got strides {x.stride()}')
+        return rows, width, ld, kind
+
+    def _check_norm(self, norm, width: int) -> tuple[int | None, int | None]:
+        if norm is None:
+            return None, None
+        w, b = norm
+        self._check(w, 'the norm weight', torch.float32, (width,))
+        self._check(b, 'the norm bias', torch.float32, (width,))
+        return w.data_ptr(), b.data_ptr()
+
+    def _call(self, name: str, *args) -> None:
+        """A library call on this device's current stream."""
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        if torch.cuda.current_device() == self.device.index:
+            self.lib.call(name, *args, stream)
+        else:
+            with torch.cuda.device(self.device):
+                self.lib.call(name, *args, stream)
+
+    def quantize_rows(self, x: torch.Tensor, norm=None) -> QuantizedRows:
+        """``x`` [rows, width] (float32, float16 or bfloat16; rows dense, any row distance) to 8-bit
+        integers with one scale per row, ``norm=(weight, bias)`` applying LayerNorm first. The
+        integers are those of the exact quotient (ties to even); ``width`` a multiple of 16."""
+        rows, width, ld, kind = self._check_rows(x)
+        w, b = self._check_norm(norm, width)
+        out = QuantizedRows(torch.empty(rows, width, dtype=torch.int8, device=self.device),
+                            torch.empty(rows, dtype=torch.float32, device=self.device))
+        args = (out.q.data_ptr(), out.scale.data_ptr(), rows, width)
+        if norm is None:
+            self._call('pq8_quantize_rows', x.data_ptr(), kind, ld, *args)
+        else:
+            self._call('pq8_layer_norm_quantize', x.data_ptr(), kind, ld, w, b, *args)
+        return out
+
+    def int8_weight(self, w) -> Int8Weight:
+        """Weights [n, k] (a float tensor, or a ``(raw, n, k)`` triple of GGUF Q8_0 bytes and its shape)
+        quantised to 8 bits with one scale per output channel."""
+        if isinstance(w, tuple):
+            raw, n, k = w
+            blocks = _host_bytes(raw).to(self.device)
+            if blocks.numel() != n * k // 32 * 34:
+                raise ValueError(f'expected {n * k // 32 * 34} Q8_0 bytes for [{n}, {k}], got {blocks.numel()}')
+            w = torch.empty(n, k, dtype=torch.float32, device=self.device)
+            self._call('pq8_dequant_q8_0', blocks.data_ptr(), w.data_ptr(), n * k)
+        rows = self.quantize_rows(w)
+        return Int8Weight(rows.q, rows.scale)
+
+    def linear_i8(self, x, w: Int8Weight, out: torch.Tensor | None = None, bias=None, resid=None,
+                  epilogue: int = EPI_NONE, alpha: float = 1.0, norm=None, out_dtype=None) -> torch.Tensor:
+        """``out = epilogue((x @ W^T) + bias)`` with the product in 8-bit integers.
+
+        ``x``: float tokens [rows, k], quantised per row on the way (after a LayerNorm with
+        ``norm=(weight, bias)``), or ``QuantizedRows``. Epilogues as ``linear``; ``EPI_GLU`` takes the
+        plain rows of ``w`` (gates in the second half). ``out_dtype``: float32 (the default),
+        float16 or bfloat16; ``out``, ``resid`` have it. ``out`` may be ``resid``, no other input."""
+        n, k = w.q.shape
+        self._check(w.q, 'the weight', torch.int8)
+        self._check(w.scale, 'the weight scale', torch.float32, (n,))
+        quantized = isinstance(x, QuantizedRows)
+        if quantized:
+            if norm is not None:
+                raise ValueError('quantised tokens take no norm')
+            rows, width = x.q.shape
+            self._check(x.q, 'x', torch.int8)
+            self._check(x.scale, 'the scale of x', torch.float32, (rows,))
+        else:
+            rows, width, ld, kind = self._check_rows(x)
+            norm_w, norm_b = self._check_norm(norm, width)
+        if width != k:
+            raise ValueError(f'x has {width} columns, weight has {k}')
+        shape = (rows, n // 2 if epilogue == EPI_GLU else n)
+        if out is None:
+            out = torch.empty(shape, dtype=out_dtype or torch.float32, device=self.device)
+        else:
+            self._check(out, 'out', out_dtype, shape)
+        y_kind = ELEMENT_TYPES.get(out.dtype)
+        if y_kind is None:
+            raise ValueError(f'the output must be float32, float16 or bfloat16, got {out.dtype}')
+        if bias is not None:
+            self._check(bias, 'bias', torch.float32, (n,))
+        if resid is not None:
+            self._check(resid, 'resid', out.dtype, shape)
+        # (the tensors stay bound here until the launch: a pointer alone would not keep their memory)
+        bias_ptr, resid_ptr = _ptr(bias), _ptr(resid)
+        if quantized:
+            self._call('pq8_gemm_i8', w.q.data_ptr(), w.scale.data_ptr(), x.q.data_ptr(), x.scale.data_ptr(),
+                       out.data_ptr(), y_kind, bias_ptr, resid_ptr, rows, n, k, epilogue, float(alpha))
+        else:
+            # scratch of this call alone: calls on other streams and captured graphs have their own
+            need = self.lib.linear_i8_workspace_size(rows, k)
+            scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
+            self._call('pq8_linear_i8', w.q.data_ptr(), w.scale.data_ptr(), x.data_ptr(), kind, ld, norm_w, norm_b,
+                       out.data_ptr(), y_kind, bias_ptr, resid_ptr, rows, n, k, epilogue, float(alpha), scratch.data_ptr(),
+                       need)
+        return out
+
+    # -- group norm --------------------------------------------------------------
+    def _check_group_norm(self, x, weight, bias, windows, offsets):
+        kind = ELEMENT_TYPES.get(x.dtype)
+        if kind is None:
+            raise ValueError(f'x must be float32, float16 or bfloat16, got {x.dtype}')
+        if x.dim() != 2:
+            raise ValueError(f'x must be a matrix, got {x.dim()} dimensions')
+        self._check(x, 'x')
+        rows, channels = x.shape
+        self._check_norm((weight, bias), channels)
+        if offsets is not None:
+            self._check(offsets, 'offsets', torch.int32, (windows + 1,))
+        elif windows < 1 or rows % windows:
+            raise ValueError(f'{rows} rows do not make {windows} windows of equal length')
+        return rows, channels, kind, None if offsets is None else offsets.data_ptr()
+
+    def group_norm(self, x: torch.Tensor, weight, bias, groups: int, windows: int = 1, offsets=None,
+                   eps: float = 1e-5, epilogue: int = EPI_NONE, flags: int = 0,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+        """Group norm and activation (``EPI_NONE``, ``EPI_RELU`` or ``EPI_SILU``), channels last: ``x``
+        [rows, channels] in ``windows`` windows of equal length, or of the rows ``offsets[i]`` to
+        ``offsets[i + 1] - 1`` (int32 on the device, ``windows + 1`` of them). Rows in no window are
+        not written: ``out`` keeps what it held, and a new tensor has nothing there."""
+        rows, channels, kind, off = self._check_group_norm(x, weight, bias, windows, offsets)
+        if out is None:
+            out = torch.empty_like(x)
+        else:
+            self._check(out, 'out', x.dtype, x.shape)
+        need = self.lib.group_norm_workspace_size(rows, windows, channels, groups)
+        scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
+        self._call('pq8_group_norm', x.data_ptr(), kind, weight.data_ptr(), bias.data_ptr(), out.data_ptr(), rows,
+                   windows, off, channels, groups, float(eps), epilogue, flags, scratch.data_ptr(), need)
+        return out
+
+    def group_norm_quantize(self, x: torch.Tensor, weight, bias, groups: int, windows: int = 1, offsets=None,
+                            eps: float = 1e-5, epilogue: int = EPI_NONE) -> QuantizedRows:
+        """``group_norm``, its rows quantised as ``quantize_rows`` does, for ``linear_i8``."""
+        rows, channels, kind, off = self._check_group_norm(x, weight, bias, windows, offsets)
+        out = QuantizedRows(torch.empty(rows, channels, dtype=torch.int8, device=self.device),
+                            torch.empty(rows, dtype=torch.float32, device=self.device))
+        need = self.lib.group_norm_workspace_size(rows, windows, channels, groups)
+        scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
+        self._call('pq8_group_norm_quantize', x.data_ptr(), kind, weight.data_ptr(), bias.data_ptr(),
+                   out.q.data_ptr(), out.scale.data_ptr(), rows, windows, off, channels, groups, float(eps), epilogue,
+                   scratch.data_ptr(), need)
         return out
 
     def device_status(self) -> int:
