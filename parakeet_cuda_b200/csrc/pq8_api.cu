@@ -2196,7 +2196,94 @@ cudaError_t launch_i8_gemv(const I8Params& p, int sms, cudaStream_t st) {
   return go(i8_gemv_kernel<T, M, 1>, 1);
 }
 
+int i8_tensor_map(EncodeTiledFn enc, CUtensorMap* map, const int8_t* base, int rows, int k, int box_rows) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(k)};
+  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)}, estr[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? PQ8_OK : PQ8_ERR_DRIVER;
+}
+
+template <typename T, int BN, bool PAIR, int STAGES>
+int launch_i8_gemm(DeviceState* ds, const I8Params& p, int splits, cudaStream_t st) {
+  using C = I8Cfg<BN, PAIR, STAGES>;
+  EncodeTiledFn enc;
+  int rc = encode_fn(&enc);
+  if (rc) return rc;
+  CUtensorMap wmap, xmap;
+  if ((rc = i8_tensor_map(enc, &wmap, p.w, p.n, p.k, p.epi == PQ8_EPI_GLU ? 16 : 128))) return rc;
+  if ((rc = i8_tensor_map(enc, &xmap, p.x, p.m, p.k, C::kTokens))) return rc;
+  I8GemmParams g{};
+  g.p = p;
+  g.n_tiles = p.epi == PQ8_EPI_GLU ? (p.out_cols + 63) / 64 : (p.n + 127) / 128;
+  g.m_tiles = (p.m + BN - 1) / BN;
+  g.k_blocks = (p.k + 127) / 128;
+  g.k_splits = splits;
+  const long long tiles = static_cast<long long>((g.n_tiles + C::kCtas - 1) / C::kCtas) * g.m_tiles;
+  if (tiles > (1 << 30)) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  const int per = splits > 1 ? splits : C::kCtas;
+  // a split CTA runs one tile (its sums take the place of the loads)
+  const long long slots = ds->sms / per;
+  if (splits > 1 && tiles > slots) return PQ8_ERR_INVALID_ARGUMENT;
+  auto kernel = i8_gemm_kernel<T, BN, PAIR, STAGES>;
+  static bool attr_set[kMaxDevices];  // guarded by g_mutex, one per kernel
+  {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return to_code(e);
+    std::lock_guard<std::mutex> lock(g_mutex);
+    if (!attr_set[dev]) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+      if (e != cudaSuccess) return to_code(e);
+      attr_set[dev] = true;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min(tiles, slots) * per));
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = per;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, wmap, xmap, g);
+  if (e != cudaSuccess) return to_code(e);
+  return to_code(cudaGetLastError());
+}
+
+// K splits for a tile count: 2, 4 or 8 CTAs a tile while they fit the SMs and
+// each keeps at least two 128-value blocks.
+int i8_splits(int tiles, int k_blocks, int sms) {
+  int s = 1;
+  while (s < 8 && tiles * s * 2 <= sms && k_blocks >= 4 * s && (2 * s - 1) * ((k_blocks + 2 * s - 1) / (2 * s)) < k_blocks)
+    s *= 2;
+  return s;
+}
+
+template <typename T>
+int launch_i8_tiles(DeviceState* ds, const I8Params& p, cudaStream_t st) {
+  const int n_tiles = p.epi == PQ8_EPI_GLU ? (p.out_cols + 63) / 64 : (p.n + 127) / 128;
+  const int k_blocks = (p.k + 127) / 128;
+  const long long tiles128 = static_cast<long long>(n_tiles) * ((p.m + 127) / 128);
+  if (tiles128 > ds->sms) return launch_i8_gemm<T, 256, true, 6>(ds, p, 1, st);
+  const int splits = i8_splits(static_cast<int>(p.m <= 64 ? n_tiles : tiles128), k_blocks, ds->sms);
+  if (p.m <= 16 && n_tiles <= ds->sms / splits) return launch_i8_gemm<T, 16, false, 8>(ds, p, splits, st);
+  if (p.m <= 32) return launch_i8_gemm<T, 32, false, 8>(ds, p, splits, st);
+  if (p.m <= 64) return launch_i8_gemm<T, 64, false, 8>(ds, p, splits, st);
+  return launch_i8_gemm<T, 128, false, 6>(ds, p, splits, st);
+}
+
 int launch_i8(DeviceState* ds, const I8Params& p, int y_type, cudaStream_t st) {
+  if (p.m > 8)
+    return with_type(y_type, [&](auto t) { return launch_i8_tiles<decltype(t)>(ds, p, st); });
   const cudaError_t e = with_type(y_type, [&](auto t) {
     using T = decltype(t);
     return p.m <= 1   ? launch_i8_gemv<T, 1>(p, ds->sms, st)

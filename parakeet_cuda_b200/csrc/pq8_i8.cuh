@@ -122,4 +122,386 @@ __global__ void __launch_bounds__(kI8GemvThreads) i8_gemv_kernel(const I8Params 
   }
 }
 
+// ---------------------------------------------------------------------------
+// More tokens: 5th-generation tensor cores, tcgen05.mma kind::i8 (8-bit operands from
+// shared memory, 32-bit integer sums in tensor memory).
+//
+// As in pq8_gemm, the MMA's M dimension is 128 weight rows and its N dimension BN
+// tokens, so an epilogue thread owns one output channel (its scale and bias
+// stay in registers) and a warp's store covers 32 consecutive channels of one
+// token: coalesced for any n, without a staging tile. Both operands are
+// K-major 128-byte rows, brought by TMA into 128-byte swizzled stages of 128
+// values of K; K past its end and rows past n or m arrive as zeros.
+//
+// PAIR: two CTAs share each MMA (cta_group::2, 256 weight rows): each loads
+// its own 128 weight rows and half of the tokens. Single CTAs may split K:
+// the S = 2, 4 or 8 CTAs of a cluster each sum a range of K, stage their sums
+// in shared memory, and add them up by bulk reductions into one another's
+// shared memory, CTA s finishing rows [s, s + 1) BN / S of the tile.
+//
+// Two accumulators let the next tile's products run under a tile's epilogue.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (and tensor-memory owner), 2 launch
+// control, 3 idle, 4-11 epilogue (two per lane quarter, half of the tokens each).
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  if constexpr (PAIR) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+// TMA load into this CTA's shared memory, counted on a barrier of the pair's leader.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];" ::"r"(smem_addr(dst)),
+      "l"(tmap), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+// Adds 32-bit integers of this CTA's shared memory to those at `dst` in a CTA of the cluster.
+__device__ __forceinline__ void bulk_add_s2s_cluster(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
+  asm volatile(
+      "cp.reduce.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes.add.s32 [%0], [%1], %2, [%3];" ::
+          "r"(dst),
+      "r"(smem_addr(src)), "r"(bytes), "r"(mbar)
+      : "memory");
+}
+
+struct I8GemmParams {
+  I8Params p;
+  int n_tiles, m_tiles, k_blocks;  // 128-row weight tiles, BN-token tiles, 128-value K blocks
+  int k_splits;
+};
+
+template <int BN_, bool PAIR_, int STAGES_>
+struct I8Cfg {
+  static constexpr int BN = BN_, STAGES = STAGES_, kCtas = PAIR_ ? 2 : 1;
+  static constexpr bool PAIR = PAIR_;
+  static constexpr int kTokens = BN / kCtas;  // token rows a CTA loads
+  static constexpr int kABytes = 128 * 128, kBBytes = kTokens * 128, kStageBytes = kABytes + kBBytes;
+  static constexpr int E = BN >= 64 ? 32 : BN / 2;  // accumulator columns per tcgen05.ld
+  static constexpr int kChunks = BN / 2 / E;        // per epilogue half
+  static constexpr int kScaleOff = STAGES * kStageBytes;  // token scales: 8 warps x 32 floats
+  static constexpr int kBarOff = kScaleOff + 8 * 32 * 4;
+  static constexpr int kNumBars = 2 * STAGES + 4 + 2;
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+  static constexpr int kSmemBytes = kMiscOff + 16 + 1024;
+  static constexpr int kTmemCols = 2 * BN <= 32 ? 32 : 2 * BN <= 64 ? 64 : 2 * BN <= 128 ? 128 : 2 * BN <= 256 ? 256 : 512;
+  static constexpr int kThreads = 12 * 32;
+  static_assert(kTokens % 8 == 0 && BN % (PAIR ? 32 : 16) == 0 && BN <= 256 && (BN / 2) % E == 0, "tile shape");
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory overflow");
+  static_assert(PAIR || BN * 128 * 4 <= STAGES * kStageBytes, "split K stages its sums in the ring");
+};
+
+template <int E>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&v)[E]) {
+  if constexpr (E == 32) tmem_ld32(taddr, v);
+  else if constexpr (E == 16) tmem_ld16(taddr, v);
+  else tmem_ld8(taddr, v);
+}
+
+template <typename T, int BN, bool PAIR, int STAGES>
+__global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
+    i8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                   const __grid_constant__ I8GemmParams g) {
+  using C = I8Cfg<BN, PAIR, STAGES>;
+  const I8Params& p = g.p;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;  // [2]
+  uint64_t* acc_empty = acc_full + 2;   // [2]
+  uint64_t* drain = acc_empty + 2;
+  uint64_t* red_full = drain + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kMiscOff + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  const bool leader = rank == 0;
+  const int S = PAIR ? 1 : g.k_splits;
+  const bool split = S > 1;
+  int* const status = p.status;
+  const bool glu = p.epi == PQ8_EPI_GLU;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 8 * C::kCtas);  // one arrival per epilogue warp
+    }
+    mbar_init(drain, 1);
+    mbar_init(red_full, 1);
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmap_w);
+    prefetch_tmap(&tmap_x);
+  }
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the peer's barriers exist before anything arrives on them
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_slot, C::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, C::kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Tiles: channel units fastest, then token tiles; the K splits of a tile are one cluster.
+  const int n_units = (g.n_tiles + C::kCtas - 1) / C::kCtas;
+  const int num_tiles = n_units * g.m_tiles;
+  const int tile0 = static_cast<int>(blockIdx.x) / (split ? S : C::kCtas);
+  const int tile_step = static_cast<int>(gridDim.x) / (split ? S : C::kCtas);
+  const int my_split = split ? static_cast<int>(cluster_rank()) : 0;
+  const int per_split = (g.k_blocks + S - 1) / S;
+  const int kb0 = my_split * per_split, kb1 = min(kb0 + per_split, g.k_blocks);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------- producer
+    if (lane == 0) {
+      griddep_wait();
+      const uint32_t full_at = PAIR ? map_to_rank(full, 0) : smem_addr(full);
+      uint32_t issued = 0;
+      Ring<STAGES> ring;
+      for (int tile = tile0; tile < num_tiles; tile += tile_step) {
+        const int unit = tile % n_units, token0 = (tile / n_units) * BN + static_cast<int>(rank) * C::kTokens;
+        const int n_tile = unit * C::kCtas + static_cast<int>(rank);
+        for (int kb = kb0; kb < kb1; ++kb, ++issued, ring.advance(1)) {
+          if (!mbar_wait(&empty[ring.idx], ring.phase ^ 1u, abort_flag, status)) goto loads_done;
+          uint8_t* a = smem + ring.idx * C::kStageBytes;
+          const uint32_t bar = full_at + ring.idx * 8;
+          if (leader) mbar_expect_tx(&full[ring.idx], C::kStageBytes * C::kCtas);
+          auto load = [&](void* dst, const void* map, int row) {
+            if constexpr (PAIR) tma_load_2d_pair(dst, map, kb * 128, row, bar);
+            else tma_load_2d(dst, map, kb * 128, row, &full[ring.idx]);
+          };
+          if (glu) {
+            // 16 rows of the first half, then the 16 gate rows of the same channels, four times
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i)
+              load(a + i * 2048, &tmap_w, ((i & 1) ? p.n / 2 : 0) + n_tile * 64 + (i >> 1) * 16);
+          } else {
+            load(a, &tmap_w, n_tile * 128);
+          }
+          load(a + C::kABytes, &tmap_x, token0);
+        }
+      }
+    loads_done:
+      // no copy may land in the shared memory of a CTA that has gone (the
+      // leader's barriers count the peer's too, and the pair leaves together)
+      if (leader)
+        for (uint32_t j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j)
+          mbar_drain(&full[j % STAGES], (j / STAGES) & 1);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (leader && lane == 0) {
+      constexpr uint32_t idesc = idesc_i8(128 * C::kCtas, BN);
+      const uint64_t desc0 = smem_desc_sw128(smem_addr(smem));
+      bool stop = false, issued = false;
+      int local = 0;
+      Ring<STAGES> ring;
+      for (int tile = tile0; tile < num_tiles && !stop; tile += tile_step, ++local) {
+        const int acc = local & 1;
+        if (!mbar_wait(&acc_empty[acc], ((local >> 1) & 1) ^ 1, abort_flag, status)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc * BN;
+        for (int kb = kb0; kb < kb1; ++kb, ring.advance(1)) {
+          if (!mbar_wait(&full[ring.idx], ring.phase, abort_flag, status)) {
+            stop = true;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t ad = desc0 + ring.idx * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_i8<PAIR>(d, ad + 2 * j, bd + 2 * j, idesc, (kb > kb0 || j > 0) ? 1u : 0u);
+          issued = true;
+          if constexpr (PAIR) mma_commit_pair(&empty[ring.idx], 0x3);
+          else mma_commit(&empty[ring.idx]);
+        }
+        if (stop) break;
+        if constexpr (PAIR) mma_commit_pair(&acc_full[acc], 0x3);
+        else mma_commit(&acc_full[acc]);
+      }
+      if (issued && *abort_flag) {  // the products under way end before the CTA is torn down
+        if constexpr (PAIR) mma_commit_pair(drain, 0x1);
+        else mma_commit(drain);
+        mbar_drain(drain, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    griddep_wait();
+    griddep_launch();
+  } else if (warp >= 4) {
+    // -------------------------------------------------------------- epilogue
+    constexpr int E = C::E;
+    const int q = warp & 3, half = (warp - 4) >> 2, r = q * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
+    float* sx = reinterpret_cast<float*>(smem + C::kScaleOff) + (warp - 4) * 32;
+    const uint32_t acc_empty_at = PAIR ? map_to_rank(acc_empty, 0) : smem_addr(acc_empty);
+    bool published = false;
+    griddep_wait();
+    int local = 0;
+    for (int tile = tile0; tile < num_tiles; tile += tile_step, ++local) {
+      const int n_tile = (tile % n_units) * C::kCtas + static_cast<int>(rank);
+      const int token0 = (tile / n_units) * BN;
+      const int acc = local & 1;
+      // this thread's channel: output column `col`, weight row `row`
+      const int col = glu ? n_tile * 64 + q * 16 + (lane & 15) : n_tile * 128 + r;
+      const int row = glu && lane >= 16 ? p.n / 2 + col : col;
+      const bool valid = col < p.out_cols;
+      const bool stores = valid && (!glu || lane < 16);
+      const float t = valid ? __ldg(p.w_scale + row) : 0.0f;
+      const float b = (valid && p.bias != nullptr) ? __ldg(p.bias + row) : 0.0f;
+      T* const y = static_cast<T*>(p.y) + col;
+      const T* const res = static_cast<const T*>(p.resid) + col;
+      const int cols = p.out_cols;
+
+      // outputs of `cnt` tokens from m0 on, whose sums are v[0 .. cnt)
+      auto finish = [&](const uint32_t(&v)[E], const T(&rv)[E], int m0, int cnt) {
+        T* yp = y + static_cast<size_t>(m0) * cols;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          float z = i8_scaled(static_cast<int>(v[j]), sx[j], t, b);
+          if (p.epi == PQ8_EPI_RESIDUAL) z = fmaf(p.alpha, z, to_f32(rv[j]));
+          else if (p.epi == PQ8_EPI_SILU) z = __fdividef(z, 1.0f + __expf(-z));
+          else if (p.epi == PQ8_EPI_RELU) z = fmaxf(z, 0.0f);
+          else if (glu) {
+            const float gate = __shfl_down_sync(0xffffffffu, z, 16);
+            z = __fdividef(z, 1.0f + __expf(-gate));
+          }
+          if (stores && j < cnt) yp[static_cast<size_t>(j) * cols] = from_f32<T>(z);
+        }
+      };
+      auto load_resid = [&](T(&rv)[E], int m0, int cnt) {
+        if (p.epi == PQ8_EPI_RESIDUAL) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) rv[j] = (stores && j < cnt) ? res[static_cast<size_t>(m0 + j) * cols] : from_f32<T>(0.0f);
+        }
+      };
+      // the scales of the tokens of a chunk, for this warp
+      auto load_scales = [&](int m0, int cnt) {
+        __syncwarp();
+        if (lane < E) sx[lane] = lane < cnt ? __ldg(p.x_scale + m0 + lane) : 0.0f;
+        __syncwarp();
+      };
+      T rv[E];
+      if (!split) {
+        const int first = token0 + half * (BN / 2);
+        load_resid(rv, first, min(E, p.m - first));
+        if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag, status)) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int cc = 0; cc < C::kChunks; ++cc) {
+          const int m0 = first + cc * E, cnt = min(E, p.m - m0);
+          uint32_t v[E];
+          tmem_ld_cols<E>(tmem + lane_base + acc * BN + half * (BN / 2) + cc * E, v);
+          load_scales(m0, cnt);
+          tmem_wait_ld();
+          if (cc + 1 == C::kChunks) {
+            tc_fence_before();
+            __syncwarp();  // every lane has read its sums: the accumulator is free
+            if (lane == 0) {
+              if (PAIR) mbar_arrive_cluster(acc_empty_at + acc * 8);
+              else mbar_arrive(&acc_empty[acc]);
+            }
+          }
+          if (cnt > 0) {
+            finish(v, rv, m0, cnt);
+            if (cc + 1 < C::kChunks) load_resid(rv, m0 + E, min(E, p.m - m0 - E));
+          }
+        }
+      } else {
+        // K split: this CTA's sums to shared memory, [token][channel] (the
+        // ring: every load has been multiplied) ...
+        int* const stage = reinterpret_cast<int*>(smem);
+        if (!mbar_wait(&acc_full[0], 0, abort_flag, status)) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int cc = 0; cc < C::kChunks; ++cc) {
+          const int c0 = half * (BN / 2) + cc * E;
+          uint32_t v[E];
+          tmem_ld_cols<E>(tmem + lane_base + c0, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < E; ++j) stage[(c0 + j) * 128 + r] = static_cast<int>(v[j]);
+        }
+        tc_fence_before();
+        fence_proxy_async_smem();  // read and added to by the bulk-copy unit
+        const int R = BN / S;      // tokens each CTA finishes
+        if (warp == 4 && lane == 0) mbar_expect_tx(red_full, static_cast<uint32_t>((S - 1) * R * 512));
+        __syncwarp();
+        cluster_sync();  // every CTA's sums are staged
+        published = true;
+        // ... then added to each finishing CTA's own, one bulk reduction each
+        if (warp == 4 && lane < S - 1) {
+          const uint32_t d = static_cast<uint32_t>((my_split + 1 + lane) % S);
+          int* src = stage + static_cast<int>(d) * R * 128;
+          bulk_add_s2s_cluster(map_to_rank(src, d), src, static_cast<uint32_t>(R * 512), map_to_rank(red_full, d));
+        }
+        __syncwarp();
+        const int rows = R / 2, off = my_split * R + half * rows;
+        const int cnt_all = min(rows, p.m - token0 - off);
+        if (!mbar_wait(red_full, 0, abort_flag, status)) break;
+#pragma unroll 1
+        for (int c0 = 0; c0 < cnt_all; c0 += E) {
+          const int cnt = min(E, cnt_all - c0), m0 = token0 + off + c0;
+          load_resid(rv, m0, cnt);
+          load_scales(m0, cnt);
+          uint32_t v[E];
+#pragma unroll
+          for (int j = 0; j < E; ++j) v[j] = j < cnt ? static_cast<uint32_t>(stage[(off + c0 + j) * 128 + r]) : 0u;
+          finish(v, rv, m0, cnt);
+        }
+      }
+    }
+    if (split && !published) {  // gave up before the sums were staged
+      __syncwarp();
+      cluster_sync();
+    }
+  }
+
+  if (split && warp < 4) {  // these warps publish nothing, but the barrier counts every thread
+    __syncwarp();
+    cluster_arrive_relaxed();
+    cluster_wait();
+  }
+  __syncthreads();
+  // The pair's MMAs read both CTAs' shared memory, and a split's sums travel
+  // between CTAs: nobody leaves before everybody is done.
+  if (PAIR || split) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, C::kTmemCols);
+    else tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
 }  // namespace pq8
