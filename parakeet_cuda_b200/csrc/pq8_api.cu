@@ -2129,28 +2129,30 @@ int check_rows_args(const void* x, int type, long long ld, const float* w, const
   return PQ8_OK;
 }
 
-template <typename T, int CHUNKS, int WARPS>
+template <typename T, int CHUNKS, int WARPS, bool VEC>
 cudaError_t launch_rows(DeviceState* ds, const T* x, long long ld, const float* w, const float* b, int8_t* q,
                         float* scale, int rows, int width, cudaStream_t st) {
   constexpr int kTeams = kRowThreads / (32 * WARPS);
-  const int vec = aligned(x, 16) && (ld * sizeof(T)) % 16 == 0;
   const dim3 grid(static_cast<unsigned>(std::min<long long>((rows + kTeams - 1LL) / kTeams, 8LL * ds->sms)));
   if (w != nullptr)
-    return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, true>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
-                      kNormEps64, q, scale, rows, width, vec);
-  return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, false>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
-                    kNormEps64, q, scale, rows, width, vec);
+    return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, true, VEC>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
+                      kNormEps64, q, scale, rows, width);
+  return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, false, VEC>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
+                    kNormEps64, q, scale, rows, width);
 }
 
 // A warp per row while 32 lanes x 32 values hold it, then a CTA per row while
-// 256 x 32 do, then rows read again in each pass.
+// 256 x 32 do; rows read again in each pass past that and where 16-byte loads
+// do not fit.
 template <typename T>
 cudaError_t launch_rows_typed(DeviceState* ds, const T* x, long long ld, const float* w, const float* b, int8_t* q,
                               float* scale, int rows, int width, cudaStream_t st) {
   constexpr int C = 32 / kChunk<T>;
-  if (width <= 1024) return launch_rows<T, C, 1>(ds, x, ld, w, b, q, scale, rows, width, st);
-  if (width <= 8192) return launch_rows<T, C, 8>(ds, x, ld, w, b, q, scale, rows, width, st);
-  return launch_rows<T, 0, 8>(ds, x, ld, w, b, q, scale, rows, width, st);
+  const bool vec = aligned(x, 16) && (rows == 1 || (ld * sizeof(T)) % 16 == 0) && aligned(w, 16) && aligned(b, 16);
+  if (!vec) return launch_rows<T, 0, 8, false>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (width <= 1024) return launch_rows<T, C, 1, true>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (width <= 8192) return launch_rows<T, C, 8, true>(ds, x, ld, w, b, q, scale, rows, width, st);
+  return launch_rows<T, 0, 8, true>(ds, x, ld, w, b, q, scale, rows, width, st);
 }
 
 int quantize_rows(const void* x, int type, long long ld, const float* w, const float* b, int8_t* q, float* scale,
@@ -2535,16 +2537,17 @@ extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, 
   const cudaError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
     GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
-    p.vec = aligned(x, 16);
+    const bool vec = aligned(x, 16) && aligned(w, 16) && aligned(b, 16);
     GroupSum* partial = static_cast<GroupSum*>(workspace);
-    cudaError_t err = launch_group_stats<T>(g, p, p.vec && (channels / groups) % kChunk<T> == 0, partial, st);
+    cudaError_t err = launch_group_stats<T>(g, p, vec && (channels / groups) % kChunk<T> == 0, partial, st);
     if (err != cudaSuccess) return err;
     const dim3 grid(g.chunks * g.slabs, g.grid_y);
-    const size_t smem = sizeof(GroupStat) * groups;
+    const size_t smem = (sizeof(GroupStat) + sizeof(float4)) * groups;
     constexpr int C = 32 / kChunk<T>;
-    auto kernel = channels <= 1024   ? group_quantize_kernel<T, C, 1>
-                  : channels <= 8192 ? group_quantize_kernel<T, C, 8>
-                                     : group_quantize_kernel<T, 0, 8>;
+    auto kernel = !vec               ? group_quantize_kernel<T, 0, 8, false>
+                  : channels <= 1024 ? group_quantize_kernel<T, C, 1, true>
+                  : channels <= 8192 ? group_quantize_kernel<T, C, 8, true>
+                                     : group_quantize_kernel<T, 0, 8, true>;
     if (smem > 48 * 1024 - 256) {
       err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
       if (err != cudaSuccess) return err;

@@ -18,7 +18,6 @@ struct GroupNormParams {
   const int* offsets;  // [windows + 1], or NULL: windows of rows / windows rows
   int rows, windows, channels, groups, epi, round_out;
   double eps;
-  int vec;         // rows of x (and y) allow 16-byte accesses, and a chunk lies within one group
   int chunks;      // row chunks per window of the sums
   int slab;        // whole groups per CTA
 };
@@ -190,37 +189,38 @@ __global__ void __launch_bounds__(kNormThreads)
 
 // Normalise, activate and quantise the rows of one chunk of one window: rows
 // whole, as their scale needs every channel.
-template <typename T, int CHUNKS, int WARPS>
-__global__ void __launch_bounds__(kRowThreads)
+template <typename T, int CHUNKS, int WARPS, bool VEC>
+__global__ void __launch_bounds__(kRowThreads, 3)
     group_quantize_kernel(const GroupNormParams p, const GroupSum* __restrict__ partial, int8_t* __restrict__ q,
                           float* __restrict__ scale) {
-  extern __shared__ GroupStat stat[];
-  __shared__ double team_smem[WARPS];
+  extern __shared__ GroupStat stat[];  // [groups], then their fp32 form
+  float4* const fast = reinterpret_cast<float4*>(stat + p.groups);
+  __shared__ double team_smem[2 * WARPS];
   __shared__ float warp_top[kRowThreads / 32];
   constexpr int kTeams = kRowThreads / (32 * WARPS);
   const RowTeam<WARPS> team{team_smem};
   griddep_wait();
   griddep_launch();
-  float top = 0.0f;
-  for (int i = threadIdx.x; i < p.channels; i += blockDim.x) top = fmaxf(top, fabsf(p.b[i]));
-  top = warp_max(top);
-  if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kRowThreads / 32; ++i) top = fmaxf(top, warp_top[i]);
-  GroupNormSource<T> src;
-  src.vec = p.vec != 0;
+  GroupNormSource<T, VEC> src;
   src.w = p.w;
   src.b = p.b;
   src.stat = stat;
+  src.fast = fast;
   src.group_width = p.channels / p.groups;
+  src.whole = src.group_width % kChunk<T> == 0;
   src.epi = p.epi;
-  src.abs = 0x1p-20f * (top + 1.0f);
+  src.top_b = cta_max_abs(p.b, p.channels, warp_top);
   for (int w = blockIdx.y; w < p.windows; w += gridDim.y) {
     int lo, hi, r0, r1;
     window_rows(p, w, &lo, &hi);
     chunk_rows(lo, hi, blockIdx.x, gridDim.x, &r0, &r1);
     group_finish<T>(p, partial, w, lo, hi, 0, p.groups, stat);
+    for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
+      const float m = static_cast<float>(stat[g].mean);
+      fast[g] = make_float4(m, static_cast<float>(stat[g].mean - static_cast<double>(m)),
+                            static_cast<float>(stat[g].rstd), 0.0f);
+    }
+    __syncthreads();
     for (int r = r0 + static_cast<int>(threadIdx.x) / (32 * WARPS); r < r1; r += kTeams) {
       src.x = static_cast<const T*>(p.x) + static_cast<size_t>(r) * p.channels;
       const float s = quantize_row<CHUNKS, WARPS>(src, p.channels, q + static_cast<size_t>(r) * p.channels, team);

@@ -196,8 +196,8 @@ struct I8Cfg {
   static constexpr int kABytes = 128 * 128, kBBytes = kTokens * 128, kStageBytes = kABytes + kBBytes;
   static constexpr int E = BN >= 64 ? 32 : BN / 2;  // accumulator columns per tcgen05.ld
   static constexpr int kChunks = BN / 2 / E;        // per epilogue half
-  static constexpr int kScaleOff = STAGES * kStageBytes;  // token scales: 8 warps x 32 floats
-  static constexpr int kBarOff = kScaleOff + 8 * 32 * 4;
+  static constexpr int kScaleOff = STAGES * kStageBytes;  // token scales of each epilogue warp's half tile
+  static constexpr int kBarOff = kScaleOff + 8 * (BN / 2) * 4;
   static constexpr int kNumBars = 2 * STAGES + 4 + 2;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kSmemBytes = kMiscOff + 16 + 1024;
@@ -213,6 +213,55 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&v)[E]) {
   if constexpr (E == 32) tmem_ld32(taddr, v);
   else if constexpr (E == 16) tmem_ld16(taddr, v);
   else tmem_ld8(taddr, v);
+}
+
+// f(the epilogue as a type): one test per chunk instead of one per output.
+template <int V>
+struct EpilogueTag {
+  static constexpr int value = V;
+};
+template <typename F>
+__device__ __forceinline__ void i8_epilogue(int epi, F&& f) {
+  if (epi == PQ8_EPI_NONE) f(EpilogueTag<PQ8_EPI_NONE>{});
+  else if (epi == PQ8_EPI_SILU) f(EpilogueTag<PQ8_EPI_SILU>{});
+  else if (epi == PQ8_EPI_RESIDUAL) f(EpilogueTag<PQ8_EPI_RESIDUAL>{});
+  else if (epi == PQ8_EPI_GLU) f(EpilogueTag<PQ8_EPI_GLU>{});
+  else f(EpilogueTag<PQ8_EPI_RELU>{});
+}
+
+// The outputs of one channel for `cnt` <= E tokens (0: this lane stores
+// nothing) from their sums v, token scales sx, channel scale t and bias b;
+// `cols` elements apart at y. Every lane of the warp takes part (GLU: the gate
+// is the channel of the lane 16 further).
+template <typename T, int E, int EPI>
+__device__ __forceinline__ void i8_finish(const uint32_t (&v)[E], const T (&rv)[E], const float* sx, float t, float b,
+                                          float alpha, T* y, int cols, int cnt) {
+  T out[E];
+#pragma unroll
+  for (int j = 0; j < E; j += 4) {
+    const float4 s4 = *reinterpret_cast<const float4*>(sx + j);
+    const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float z = i8_scaled(static_cast<int>(v[j + i]), s[i], t, b);
+      if constexpr (EPI == PQ8_EPI_RESIDUAL) z = fmaf(alpha, z, to_f32(rv[j + i]));
+      if constexpr (EPI == PQ8_EPI_SILU) z = __fdividef(z, 1.0f + __expf(-z));
+      if constexpr (EPI == PQ8_EPI_RELU) z = fmaxf(z, 0.0f);
+      if constexpr (EPI == PQ8_EPI_GLU) {
+        const float gate = __shfl_down_sync(0xffffffffu, z, 16);
+        z = __fdividef(z, 1.0f + __expf(-gate));
+      }
+      out[j + i] = from_f32<T>(z);
+    }
+  }
+  if (cnt == E) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) y[static_cast<size_t>(j) * cols] = out[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (j < cnt) y[static_cast<size_t>(j) * cols] = out[j];
+  }
 }
 
 template <typename T, int BN, bool PAIR, int STAGES>
@@ -364,7 +413,7 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
     constexpr int E = C::E;
     const int q = warp & 3, half = (warp - 4) >> 2, r = q * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
-    float* sx = reinterpret_cast<float*>(smem + C::kScaleOff) + (warp - 4) * 32;
+    float* sx = reinterpret_cast<float*>(smem + C::kScaleOff) + (warp - 4) * (BN / 2);
     const uint32_t acc_empty_at = PAIR ? map_to_rank(acc_empty, 0) : smem_addr(acc_empty);
     bool published = false;
     griddep_wait();
@@ -385,20 +434,11 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
       const int cols = p.out_cols;
 
       // outputs of `cnt` tokens from m0 on, whose sums are v[0 .. cnt)
-      auto finish = [&](const uint32_t(&v)[E], const T(&rv)[E], int m0, int cnt) {
-        T* yp = y + static_cast<size_t>(m0) * cols;
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          float z = i8_scaled(static_cast<int>(v[j]), sx[j], t, b);
-          if (p.epi == PQ8_EPI_RESIDUAL) z = fmaf(p.alpha, z, to_f32(rv[j]));
-          else if (p.epi == PQ8_EPI_SILU) z = __fdividef(z, 1.0f + __expf(-z));
-          else if (p.epi == PQ8_EPI_RELU) z = fmaxf(z, 0.0f);
-          else if (glu) {
-            const float gate = __shfl_down_sync(0xffffffffu, z, 16);
-            z = __fdividef(z, 1.0f + __expf(-gate));
-          }
-          if (stores && j < cnt) yp[static_cast<size_t>(j) * cols] = from_f32<T>(z);
-        }
+      auto finish = [&](const uint32_t(&v)[E], const T(&rv)[E], const float* sx, int m0, int cnt) {
+        T* const yp = y + static_cast<size_t>(m0) * cols;
+        i8_epilogue(p.epi, [&](auto epi) {
+          i8_finish<T, E, decltype(epi)::value>(v, rv, sx, t, b, p.alpha, yp, cols, stores ? cnt : 0);
+        });
       };
       auto load_resid = [&](T(&rv)[E], int m0, int cnt) {
         if (p.epi == PQ8_EPI_RESIDUAL) {
@@ -406,15 +446,18 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
           for (int j = 0; j < E; ++j) rv[j] = (stores && j < cnt) ? res[static_cast<size_t>(m0 + j) * cols] : from_f32<T>(0.0f);
         }
       };
-      // the scales of the tokens of a chunk, for this warp
-      auto load_scales = [&](int m0, int cnt) {
-        __syncwarp();
-        if (lane < E) sx[lane] = lane < cnt ? __ldg(p.x_scale + m0 + lane) : 0.0f;
+      // the scales of up to BN / 2 tokens from m0 on, for this warp
+      auto load_scales = [&](int m0) {
+        __syncwarp();  // the previous tile's have been read
+#pragma unroll
+        for (int i = 0; i < BN / 2; i += 32)
+          if (i + lane < BN / 2) sx[i + lane] = m0 + i + lane < p.m ? __ldg(p.x_scale + m0 + i + lane) : 0.0f;
         __syncwarp();
       };
       T rv[E];
       if (!split) {
         const int first = token0 + half * (BN / 2);
+        load_scales(first);
         load_resid(rv, first, min(E, p.m - first));
         if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag, status)) break;
         tc_fence_after();
@@ -423,7 +466,6 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
           const int m0 = first + cc * E, cnt = min(E, p.m - m0);
           uint32_t v[E];
           tmem_ld_cols<E>(tmem + lane_base + acc * BN + half * (BN / 2) + cc * E, v);
-          load_scales(m0, cnt);
           tmem_wait_ld();
           if (cc + 1 == C::kChunks) {
             tc_fence_before();
@@ -434,7 +476,7 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
             }
           }
           if (cnt > 0) {
-            finish(v, rv, m0, cnt);
+            finish(v, rv, sx + cc * E, m0, cnt);
             if (cc + 1 < C::kChunks) load_resid(rv, m0 + E, min(E, p.m - m0 - E));
           }
         }
@@ -469,16 +511,16 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
         __syncwarp();
         const int rows = R / 2, off = my_split * R + half * rows;
         const int cnt_all = min(rows, p.m - token0 - off);
+        load_scales(token0 + off);
         if (!mbar_wait(red_full, 0, abort_flag, status)) break;
 #pragma unroll 1
         for (int c0 = 0; c0 < cnt_all; c0 += E) {
           const int cnt = min(E, cnt_all - c0), m0 = token0 + off + c0;
           load_resid(rv, m0, cnt);
-          load_scales(m0, cnt);
           uint32_t v[E];
 #pragma unroll
           for (int j = 0; j < E; ++j) v[j] = j < cnt ? static_cast<uint32_t>(stage[(off + c0 + j) * 128 + r]) : 0u;
-          finish(v, rv, m0, cnt);
+          finish(v, rv, sx + c0, m0, cnt);
         }
       }
     }

@@ -18,6 +18,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "pq8_block.cuh"
 #include "pq8_device.cuh"
 
@@ -62,6 +64,36 @@ __device__ __forceinline__ void load_chunk(const T* p, bool vec, float (&v)[E]) 
     for (int i = 0; i < E; ++i) v[i] = to_f32(p[i]);
   }
 }
+// `E` consecutive floats of a parameter vector (E a multiple of 4; column of
+// a chunk, so 16-byte aligned when the vector is).
+template <int E>
+__device__ __forceinline__ void load_params(const float* p, bool vec, float (&v)[E]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(p + i));
+      v[i] = u.x;
+      v[i + 1] = u.y;
+      v[i + 2] = u.z;
+      v[i + 3] = u.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = __ldg(p + i);
+  }
+}
+// The largest |b[i]| of a vector, by every thread of the CTA for itself.
+__device__ __forceinline__ float cta_max_abs(const float* b, int n, float* smem /* a float per warp */) {
+  float top = 0.0f;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) top = fmaxf(top, fabsf(b[i]));
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = smem[0];
+  for (int i = 1; i < static_cast<int>(blockDim.x >> 5); ++i) top = fmaxf(top, smem[i]);
+  return top;
+}
+
 template <typename T, int E>
 __device__ __forceinline__ void store_chunk(T* p, bool vec, const float (&v)[E]) {
   if (vec) {
@@ -91,28 +123,52 @@ __device__ __forceinline__ double warp_max_f64(double v) {
 // order (lanes by butterfly, then warps in turn).
 template <int WARPS>
 struct RowTeam {
-  double* smem;  // WARPS doubles, when WARPS > 1
+  double* smem;  // 2 WARPS doubles, when WARPS > 1
   __device__ __forceinline__ int index() const { return WARPS == 1 ? (threadIdx.x & 31) : static_cast<int>(threadIdx.x); }
-  __device__ __forceinline__ double gather(double v, bool sum) const {
-    if constexpr (WARPS == 1) {
-      return v;
-    } else {
+  __device__ __forceinline__ void sum2(double& a, double& b) const {
+    a = warp_sum_f64(a);
+    b = warp_sum_f64(b);
+    if constexpr (WARPS > 1) {
       __syncthreads();  // the previous reduction has been read
-      if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
+      if ((threadIdx.x & 31) == 0) {
+        smem[2 * (threadIdx.x >> 5)] = a;
+        smem[2 * (threadIdx.x >> 5) + 1] = b;
+      }
       __syncthreads();
-      double r = smem[0];
+      a = smem[0];
+      b = smem[1];
 #pragma unroll
-      for (int i = 1; i < WARPS; ++i) r = sum ? r + smem[i] : fmax(r, smem[i]);
-      return r;
+      for (int i = 1; i < WARPS; ++i) {
+        a += smem[2 * i];
+        b += smem[2 * i + 1];
+      }
     }
   }
-  __device__ __forceinline__ double sum(double v) const { return gather(warp_sum_f64(v), true); }
-  __device__ __forceinline__ double max(double v) const { return gather(warp_max_f64(v), false); }
-  __device__ __forceinline__ float max(float v) const {
-    return WARPS == 1 ? warp_max(v) : static_cast<float>(gather(static_cast<double>(warp_max(v)), false));
+  __device__ __forceinline__ double max(double v) const {
+    v = warp_max_f64(v);
+    if constexpr (WARPS > 1) {
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = smem[0];
+#pragma unroll
+      for (int i = 1; i < WARPS; ++i) v = fmax(v, smem[i]);
+    }
+    return v;
   }
-  __device__ __forceinline__ bool any(bool p) const {
-    return WARPS == 1 ? __any_sync(0xffffffffu, p) : __syncthreads_or(p) != 0;
+  // of values >= 0 (infinity included), whose bit patterns are ordered as they are
+  __device__ __forceinline__ float max(float v) const {
+    v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+    if constexpr (WARPS > 1) {
+      float* f = reinterpret_cast<float*>(smem);
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) f[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = f[0];
+#pragma unroll
+      for (int i = 1; i < WARPS; ++i) v = fmaxf(v, f[i]);
+    }
+    return v;
   }
 };
 
@@ -128,110 +184,72 @@ __device__ __forceinline__ float act_f32(float z, int epi) {
 }
 
 // ---------------------------------------------------------------------------
-// Where a row's values come from. A source gives, for a chunk of columns, the
-// fp32 values, whose error against the exact ones is at most
-// rel |value| + abs; and the exact value of one column in fp64.
+// Where a row's values come from (VEC: by 16-byte loads, of the row and of the
+// norm's parameters). A source gives, for a chunk of columns, the
+// fp32 values, whose error against the exact ones is at
+// most error(h) for values up to h; and the exact value of one column in fp64.
 
 // The row itself: nothing to compute, no error.
-template <typename T>
+template <typename T, bool VEC>
 struct PlainSource {
   static constexpr bool kExact = true, kLayerNorm = false;
   static constexpr int E = kChunk<T>;
   const T* x;
-  bool vec;
-  float rel = 0.0f, abs = 0.0f;
-  __device__ __forceinline__ void raw(int c, float (&v)[E]) const { load_chunk<T, E>(x + c * E, vec, v); }
-  template <typename Team>
-  __device__ __forceinline__ void prepare(const Team&, int, const float*, int) {}
+  __device__ __forceinline__ void raw(int c, float (&v)[E]) const { load_chunk<T, E>(x + c * E, VEC, v); }
   __device__ __forceinline__ void value(int, float (&)[E]) const {}
   __device__ __forceinline__ double exact(int col) const { return static_cast<double>(to_f32(x[col])); }
+  __device__ __forceinline__ float error(float) const { return 0.0f; }
 };
 
 // LayerNorm of the row. fp32 error: the deviation (x - mean_hi) - mean_lo is
 // rounded twice relative to its own size (the mean's own rounding is in
 // mean_lo), then one rounding each for rstd, the product and the multiply-add:
 // under 6 x 2^-24 (|h| + |b|), taken as 2^-21.
-template <typename T>
+template <typename T, bool VEC>
 struct LayerNormSource {
   static constexpr bool kExact = false, kLayerNorm = true;
   static constexpr int E = kChunk<T>;
   const T* x;
-  bool vec;
   const float* w;
   const float* b;
-  double eps;
-  float rel = 0x1p-21f, abs = 0.0f;
-  double mean = 0.0, rstd = 0.0;
-  float mean_hi = 0.0f, mean_lo = 0.0f, rs = 0.0f;
-  __device__ __forceinline__ void raw(int c, float (&v)[E]) const { load_chunk<T, E>(x + c * E, vec, v); }
-  // Mean and variance of the row: from the chunks held in `cached` (chunk
-  // index + j * team size), or read again when cached is NULL.
-  template <typename Team, int CHUNKS>
-  __device__ __forceinline__ void stats(const Team& team, int threads, const float (&cached)[CHUNKS * E], int chunks) {
-    const int tid = team.index();
-    double s = 0.0;
+  double eps, inv_width;
+  float top_b;  // max|b|
+  double mean, rstd;
+  float mean_hi, mean_lo, rs;
+  __device__ __forceinline__ void raw(int c, float (&v)[E]) const { load_chunk<T, E>(x + c * E, VEC, v); }
+  // Sums of x - first and its square: with a value of the row taken off, the
+  // square of the mean is at most `width` times the variance, so their
+  // difference keeps all but three or four of fp64's digits.
+  __device__ __forceinline__ void add(const float (&v)[E], double first, double& s, double& q) const {
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j)
-      if (tid + j * threads < chunks) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) s += static_cast<double>(cached[j * E + i]);
-      }
-    mean = team.sum(s) / (static_cast<double>(chunks) * E);
-    double q = 0.0;
-    float bm = 0.0f;
-#pragma unroll
-    for (int j = 0; j < CHUNKS; ++j)
-      if (tid + j * threads < chunks) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const double d = static_cast<double>(cached[j * E + i]) - mean;
-          q += d * d;
-          bm = fmaxf(bm, fabsf(b[(tid + j * threads) * E + i]));
-        }
-      }
-    finish(team, q, bm, chunks);
+    for (int i = 0; i < E; ++i) {
+      const double d = static_cast<double>(v[i]) - first;
+      s += d;
+      q += d * d;
+    }
   }
   template <typename Team>
-  __device__ __forceinline__ void stats_streamed(const Team& team, int threads, int chunks) {
-    const int tid = team.index();
-    double s = 0.0;
-    float v[E];
-    for (int c = tid; c < chunks; c += threads) {
-      raw(c, v);
-#pragma unroll
-      for (int i = 0; i < E; ++i) s += static_cast<double>(v[i]);
-    }
-    mean = team.sum(s) / (static_cast<double>(chunks) * E);
-    double q = 0.0;
-    float bm = 0.0f;
-    for (int c = tid; c < chunks; c += threads) {
-      raw(c, v);
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const double d = static_cast<double>(v[i]) - mean;
-        q += d * d;
-        bm = fmaxf(bm, fabsf(b[c * E + i]));
-      }
-    }
-    finish(team, q, bm, chunks);
-  }
-  template <typename Team>
-  __device__ __forceinline__ void finish(const Team& team, double q, float bm, int chunks) {
-    rstd = 1.0 / sqrt(team.sum(q) / (static_cast<double>(chunks) * E) + eps);
-    abs = 0x1p-21f * team.max(bm);
+  __device__ __forceinline__ void finish(const Team& team, double first, double s, double q) {
+    team.sum2(s, q);
+    const double m = s * inv_width;
+    mean = first + m;
+    rstd = rsqrt(fmax(q * inv_width - m * m, 0.0) + eps);
     mean_hi = static_cast<float>(mean);
     mean_lo = static_cast<float>(mean - static_cast<double>(mean_hi));
     rs = static_cast<float>(rstd);
   }
   __device__ __forceinline__ void value(int c, float (&v)[E]) const {
+    float g[E], h[E];
+    load_params<E>(w + c * E, VEC, g);
+    load_params<E>(b + c * E, VEC, h);
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-      v[i] = fmaf(((v[i] - mean_hi) - mean_lo) * rs, __ldg(w + c * E + i), __ldg(b + c * E + i));
+    for (int i = 0; i < E; ++i) v[i] = fmaf(((v[i] - mean_hi) - mean_lo) * rs, g[i], h[i]);
   }
   __device__ __forceinline__ double exact(int col) const {
     return (static_cast<double>(to_f32(x[col])) - mean) * rstd * static_cast<double>(w[col]) +
            static_cast<double>(b[col]);
   }
+  __device__ __forceinline__ float error(float h) const { return 0x1p-21f * (h + top_b); }
 };
 
 // Group norm with its activation; mean and 1 / sqrt(var + eps) of the row's
@@ -240,35 +258,34 @@ struct LayerNormSource {
 struct GroupStat {
   double mean, rstd;
 };
-template <typename T>
+template <typename T, bool VEC>
 struct GroupNormSource {
   static constexpr bool kExact = false, kLayerNorm = false;
   static constexpr int E = kChunk<T>;
   const T* x;
-  bool vec;
   const float* w;
   const float* b;
   const GroupStat* stat;  // [groups], shared memory
+  const float4* fast;     // [groups], shared memory: mean's high and low part, 1 / deviation in fp32
   int group_width;
+  bool whole;             // a chunk lies within one group
   int epi;
-  float rel = 0x1p-20f, abs;  // abs = 2^-20 (max|b| + 1)
-  __device__ __forceinline__ void raw(int c, float (&v)[E]) const { load_chunk<T, E>(x + c * E, vec, v); }
+  float top_b;  // max|b|
+  __device__ __forceinline__ void raw(int c, float (&v)[E]) const { load_chunk<T, E>(x + c * E, VEC, v); }
   __device__ __forceinline__ void value(int c, float (&v)[E]) const {
-    int g = c * E / group_width, left = (g + 1) * group_width - c * E;
-    GroupStat s = stat[g];
-    float hi = static_cast<float>(s.mean), lo = static_cast<float>(s.mean - static_cast<double>(hi));
-    float rs = static_cast<float>(s.rstd);
+    float g[E], h[E];
+    load_params<E>(w + c * E, VEC, g);
+    load_params<E>(b + c * E, VEC, h);
+    if (whole) {
+      const float4 f = fast[c * E / group_width];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      if (left == 0) {
-        s = stat[++g];
-        left = group_width;
-        hi = static_cast<float>(s.mean);
-        lo = static_cast<float>(s.mean - static_cast<double>(hi));
-        rs = static_cast<float>(s.rstd);
+      for (int i = 0; i < E; ++i) v[i] = act_f32(fmaf(((v[i] - f.x) - f.y) * f.z, g[i], h[i]), epi);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float4 f = fast[(c * E + i) / group_width];
+        v[i] = act_f32(fmaf(((v[i] - f.x) - f.y) * f.z, g[i], h[i]), epi);
       }
-      --left;
-      v[i] = act_f32(fmaf(((v[i] - hi) - lo) * rs, __ldg(w + c * E + i), __ldg(b + c * E + i)), epi);
     }
   }
   __device__ __forceinline__ double exact(int col) const {
@@ -277,6 +294,7 @@ struct GroupNormSource {
                      static_cast<double>(b[col]);
     return act_f64(z, epi);
   }
+  __device__ __forceinline__ float error(float h) const { return 0x1p-20f * (h + top_b + 1.0f); }
 };
 
 // ---------------------------------------------------------------------------
@@ -284,116 +302,134 @@ struct GroupNormSource {
 // chunks of the row in registers (width <= CHUNKS * E * 32 * WARPS);
 // CHUNKS == 0: any width, read again in each pass. `width` is a multiple of
 // E; q is E-byte aligned. Every thread of the team returns the scale.
+//
+// Per value, the common path is a multiply-add that rounds (adding 1.5 x
+// 2^23 leaves the nearest integer in the low bits), its remainder, and a
+// running maximum of the remainders: a thread looks its values through for
+// the ones next to a border only when that maximum says there is one.
 template <int CHUNKS, int WARPS, typename Src>
 __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, const RowTeam<WARPS>& team) {
   constexpr int E = Src::E;
   constexpr int kThreads = WARPS * 32;
   constexpr bool kCached = CHUNKS > 0;
   constexpr int N = kCached ? CHUNKS : 1;
-  static_assert(!kCached || N * E <= 32, "one mask bit per value");
   const int tid = team.index(), chunks = width / E;
-  float v[N * E];
+  static_assert(N * E <= 32, "a mask bit per value");
+  float v[N][E];
   if constexpr (kCached) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      float c4[E];
       const int c = tid + j * kThreads;
-      if (c < chunks) src.raw(c, c4);
-#pragma unroll
-      for (int i = 0; i < E; ++i) v[j * E + i] = c < chunks ? c4[i] : 0.0f;
+      if (c < chunks) src.raw(c, v[j]);
     }
-    if constexpr (Src::kLayerNorm) src.template stats<RowTeam<WARPS>, N>(team, kThreads, v, chunks);
-  } else {
-    if constexpr (Src::kLayerNorm) src.stats_streamed(team, kThreads, chunks);
   }
-  // f(first register, chunk) for every chunk of this thread
+  // f(values, chunk) for every chunk of this thread; `compute`: from the raw
+  // ones (rows that are not cached always start from those)
   auto each = [&](auto&& f, bool compute) {
     if constexpr (kCached) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const int c = tid + j * kThreads;
         if (c < chunks) {
-          float(&c4)[E] = *reinterpret_cast<float(*)[E]>(v + j * E);
-          if (compute) src.value(c, c4);
-          f(c4, c, j * E);
+          if (compute) src.value(c, v[j]);
+          f(v[j], c);
         }
       }
     } else {
       for (int c = tid; c < chunks; c += kThreads) {
-        float(&c4)[E] = *reinterpret_cast<float(*)[E]>(v);
-        src.raw(c, c4);
-        src.value(c, c4);
-        f(c4, c, 0);
+        src.raw(c, v[0]);
+        src.value(c, v[0]);
+        f(v[0], c);
       }
     }
   };
-  // column of mask bit `bit` (cached rows)
-  auto column = [&](int bit) { return (tid + (bit / E) * kThreads) * E + bit % E; };
+  // f(column) for the columns of this thread whose value `pick`s: those are
+  // found in registers, then taken one at a time
+  auto columns = [&](auto&& pick, auto&& f) {
+    uint32_t found = 0;
+    auto pick_chunk = [&](const float(&u)[E]) {
+      uint32_t here = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) here |= pick(u[i]) ? 1u << i : 0u;
+      return here;
+    };
+    if constexpr (kCached) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (tid + j * kThreads < chunks) found |= pick_chunk(v[j]) << (j * E);
+      for (; found; found &= found - 1) {
+        const int bit = __ffs(found) - 1;
+        f((tid + (bit / E) * kThreads) * E + bit % E);
+      }
+    } else {
+#pragma unroll 1
+      for (int c = tid; c < chunks; c += kThreads) {
+        src.raw(c, v[0]);
+        src.value(c, v[0]);
+        for (found = pick_chunk(v[0]); found; found &= found - 1) f(c * E + __ffs(found) - 1);
+      }
+    }
+  };
+  if constexpr (Src::kLayerNorm) {
+    const double first = static_cast<double>(to_f32(src.x[0]));
+    double s = 0.0, sq = 0.0;
+    if constexpr (kCached) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (tid + j * kThreads < chunks) src.add(v[j], first, s, sq);
+    } else {
+      for (int c = tid; c < chunks; c += kThreads) {
+        src.raw(c, v[0]);
+        src.add(v[0], first, s, sq);
+      }
+    }
+    src.finish(team, first, s, sq);
+  }
 
-  float low = 0.0f;  // a lower bound on the row's maximum
-  bool bad = false;
-  each([&](const float(&c4)[E], int, int) {
+  float mine = 0.0f, bad = 0.0f;
+  each([&](const float(&u)[E], int) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float a = fabsf(c4[i]);
-      bad |= !(a <= 3.402823466e38f);
-      low = fmaxf(low, a - (src.rel * a + src.abs));
+      mine = fmaxf(mine, fabsf(u[i]));
+      bad = fmaf(u[i], 0.0f, bad);  // NaN from an infinity or a NaN on
     }
   }, true);
-  auto zeros = [&] {
+  const float top = team.max(bad == 0.0f ? mine : INFINITY);
+  float s = top / 127.0f;
+  if constexpr (!Src::kExact) {
+    if (top < INFINITY) {
+      // the values that may be the largest, exactly
+      const float least = top - 2.5f * src.error(top);
+      double t64 = 0.0;
+      if (mine >= least)
+        columns([&](float u) { return fabsf(u) >= least; },
+                [&](int col) { t64 = fmax(t64, ::fabs(src.exact(col))); });
+      s = static_cast<float>(team.max(t64) * (1.0 / 127.0));
+    }
+  }
+  if (!(top < INFINITY) || s == 0.0f) {
+    // an infinity or a NaN in the row: no scale, no values; a row of zeros, or
+    // of values too small for a scale: zeros
     for (int c = tid; c < chunks; c += kThreads)
 #pragma unroll
       for (int i = 0; i < E; i += 4) *reinterpret_cast<uint32_t*>(q + c * E + i) = 0u;
-  };
-  if (team.any(bad)) {  // an infinity or a NaN in the row: no scale, no values
-    zeros();
-    return __int_as_float(0x7fc00000);
+    return top < INFINITY ? 0.0f : __int_as_float(0x7fc00000);
   }
-  low = team.max(low);
-  float s;
-  if constexpr (Src::kExact) {
-    s = low / 127.0f;
-  } else {
-    double top = 0.0;
-    uint32_t near = 0;
-    each([&](const float(&c4)[E], int c, int bit) {
-      uint32_t here = 0;
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const float a = fabsf(c4[i]);
-        if (a + (src.rel * a + src.abs) >= low) here |= 1u << i;
-      }
-      if constexpr (kCached) {
-        near |= here << bit;
-      } else {
-        for (; here; here &= here - 1) top = fmax(top, ::fabs(src.exact(c * E + __ffs(here) - 1)));
-      }
-    }, false);
-    for (; near; near &= near - 1) top = fmax(top, ::fabs(src.exact(column(__ffs(near) - 1))));
-    s = static_cast<float>(team.max(top) / 127.0);
-  }
-  if (s == 0.0f) {  // a row of zeros, or of values too small for a scale
-    zeros();
-    return 0.0f;
-  }
-  const double s64 = static_cast<double>(s);
-  const float inv = 1.0f / s;
+  const float inv = __fdividef(1.0f, s);  // off by at most 2^-22: in `border`
+  constexpr float kBig = 12582912.0f;
   // below this, 1 / s may leave fp32's range: every quotient in fp64
-  const bool all_exact = s < 0x1p-100f;
-  const float tol_rel = src.rel + 0x1p-22f, tol_abs = src.abs * inv;
-  auto exact_q = [&](int col) {
-    return static_cast<int8_t>(static_cast<int>(fmin(fmax(rint(src.exact(col) / s64), -127.0), 127.0)));
-  };
-  uint32_t fix = 0;
-  each([&](const float(&c4)[E], int c, int bit) {
-    uint32_t here = 0, m[E], word[E / 4];
+  const bool all = s < 0x1p-100f;
+  // |remainder| from which a quotient may lie on the other side of a border:
+  // the value's error, and that of the reciprocal and the product
+  const float border = 0.5f - (128.0f * 0x1p-21f + src.error(top) * inv);
+  float worst = 0.0f;
+  each([&](const float(&u)[E], int c) {
+    uint32_t m[E], word[E / 4];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      // adding 1.5 x 2^23 rounds to an integer (nearest even) and leaves it in the low bits
-      const float t = c4[i] * inv, big = t + 12582912.0f, r = big - 12582912.0f;
+      const float big = fmaf(u[i], inv, kBig);
       m[i] = __float_as_uint(big);
-      // not (|t - r| below the border by more than the error), NaN included
-      if (!(fabsf(t - r) < 0.5f - fmaf(fabsf(t), tol_rel, tol_abs)) || all_exact) here |= 1u << i;
+      worst = fmaxf(worst, fabsf(fmaf(u[i], inv, kBig - big)));
     }
 #pragma unroll
     for (int i = 0; i < E; i += 4)
@@ -403,18 +439,17 @@ __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, con
     } else {
       *reinterpret_cast<uint2*>(q + c * E) = make_uint2(word[0], word[E / 4 - 1]);
     }
-    if constexpr (kCached) {
-      fix |= here << bit;
-    } else {
-      for (; here; here &= here - 1) {
-        const int col = c * E + __ffs(here) - 1;
-        q[col] = exact_q(col);
-      }
-    }
   }, false);
-  for (; fix; fix &= fix - 1) {
-    const int col = column(__ffs(fix) - 1);
-    q[col] = exact_q(col);
+  if (worst >= border || all) {
+    const double s64 = static_cast<double>(s);
+    columns(
+        [&](float u) {
+          const float big = fmaf(u, inv, kBig);
+          return all || fabsf(fmaf(u, inv, kBig - big)) >= border;
+        },
+        [&](int col) {
+          q[col] = static_cast<int8_t>(static_cast<int>(fmin(fmax(rint(src.exact(col) / s64), -127.0), 127.0)));
+        });
   }
   return s;
 }
@@ -423,37 +458,32 @@ constexpr int kRowThreads = 256;
 
 // Rows of a [rows, width] matrix (row stride ld elements), each quantised by
 // a team of WARPS warps: a warp per row up to 1024 columns, the CTA's eight
-// warps up to 8192 (the row stays in registers in both), and past that the
-// CTA reads the row again in each pass. NORM: LayerNorm first.
-template <typename T, int CHUNKS, int WARPS, bool NORM>
-__global__ void __launch_bounds__(kRowThreads)
+// warps up to 8192 (the row stays in registers in both), and past that, or
+// where 16-byte loads do not fit, the CTA reads the row again in each pass.
+// NORM: LayerNorm first.
+template <typename T, int CHUNKS, int WARPS, bool NORM, bool VEC>
+__global__ void __launch_bounds__(kRowThreads, NORM ? 3 : 4)
     quantize_rows_kernel(const T* __restrict__ x, long long ld, const float* __restrict__ w,
                          const float* __restrict__ b, double eps, int8_t* __restrict__ q, float* __restrict__ scale,
-                         int rows, int width, int vec) {
-  __shared__ double team_smem[WARPS];
+                         int rows, int width) {
+  __shared__ double team_smem[2 * WARPS];
+  __shared__ float top_smem[kRowThreads / 32];
   constexpr int kTeams = kRowThreads / (32 * WARPS);
   const RowTeam<WARPS> team{team_smem};
   griddep_wait();    // x is the previous kernel's output
   griddep_launch();  // only now: what the next kernel reads ahead of its own wait is then older than this kernel
+  std::conditional_t<NORM, LayerNormSource<T, VEC>, PlainSource<T, VEC>> src;
+  if constexpr (NORM) {
+    src.w = w;
+    src.b = b;
+    src.eps = eps;
+    src.inv_width = 1.0 / width;
+    src.top_b = cta_max_abs(b, width, top_smem);
+  }
   const int first = static_cast<int>(blockIdx.x) * kTeams + static_cast<int>(threadIdx.x) / (32 * WARPS);
   for (long long row = first; row < rows; row += static_cast<long long>(gridDim.x) * kTeams) {
-    const T* xr = x + row * ld;
-    int8_t* qr = q + row * width;
-    float s;
-    if constexpr (NORM) {
-      LayerNormSource<T> src;
-      src.x = xr;
-      src.vec = vec != 0;
-      src.w = w;
-      src.b = b;
-      src.eps = eps;
-      s = quantize_row<CHUNKS, WARPS>(src, width, qr, team);
-    } else {
-      PlainSource<T> src;
-      src.x = xr;
-      src.vec = vec != 0;
-      s = quantize_row<CHUNKS, WARPS>(src, width, qr, team);
-    }
+    src.x = x + row * ld;
+    const float s = quantize_row<CHUNKS, WARPS>(src, width, q + row * width, team);
     if (team.index() == 0) scale[row] = s;
   }
 }
