@@ -2185,17 +2185,36 @@ int check_i8_args(const int8_t* w, const float* w_scale, const void* y, int y_ty
   return PQ8_OK;
 }
 
-template <typename T, int M>
-cudaError_t launch_i8_gemv(const I8Params& p, int sms, cudaStream_t st) {
+// Channels per warp: as many as keep every SM at two CTAs or more.
+template <int M, bool FUSED, typename T, bool NORM>
+cudaError_t launch_i8_gemv(const I8Params& p, const I8Tokens& tokens, int y_type, int sms, cudaStream_t st) {
   const int warps = kI8GemvThreads / 32;
   const bool glu = p.epi == PQ8_EPI_GLU;
   auto go = [&](auto kernel, int per_warp) {
-    const dim3 grid((p.out_cols + per_warp * warps - 1) / (per_warp * warps), std::min((p.m + M - 1) / M, 32768));
-    return launch_pdl(kernel, grid, dim3(kI8GemvThreads), 0, st, p);
+    const dim3 grid((p.out_cols + per_warp * warps - 1) / (per_warp * warps));
+    return launch_pdl(kernel, grid, dim3(kI8GemvThreads), FUSED ? static_cast<size_t>(p.m) * p.k : 0, st, p, tokens,
+                      y_type);
   };
-  if (p.n >= 4 * warps * sms) return go(i8_gemv_kernel<T, M, 4>, glu ? 2 : 4);
-  if (p.n >= 2 * warps * sms || glu) return go(i8_gemv_kernel<T, M, 2>, glu ? 1 : 2);
-  return go(i8_gemv_kernel<T, M, 1>, 1);
+  if (p.n >= 4 * warps * sms) return go(i8_gemv_kernel<M, 4, FUSED, T, NORM>, glu ? 2 : 4);
+  if (p.n >= 2 * warps * sms || glu) return go(i8_gemv_kernel<M, 2, FUSED, T, NORM>, glu ? 1 : 2);
+  return go(i8_gemv_kernel<M, 1, FUSED, T, NORM>, 1);
+}
+
+// m <= 8. `tokens` in floating point (FUSED), or p.x quantised.
+template <bool FUSED, typename T, bool NORM>
+int launch_i8_few(DeviceState* ds, const I8Params& p, const I8Tokens& tokens, int y_type, cudaStream_t st) {
+  const cudaError_t e = p.m <= 1   ? launch_i8_gemv<1, FUSED, T, NORM>(p, tokens, y_type, ds->sms, st)
+                        : p.m <= 4 ? launch_i8_gemv<4, FUSED, T, NORM>(p, tokens, y_type, ds->sms, st)
+                                   : launch_i8_gemv<8, FUSED, T, NORM>(p, tokens, y_type, ds->sms, st);
+  if (e != cudaSuccess) return to_code(e);
+  return to_code(cudaGetLastError());
+}
+
+// Whether the GEMV quantises the tokens itself: rows that its teams hold in
+// registers, read by 16-byte loads.
+bool i8_fused(const void* x, int type, long long ld, const float* norm_w, const float* norm_b, int m, int k) {
+  return m <= kI8GemvMaxM && k <= (m == 1 ? 8192 : 1024) && aligned(x, 16) &&
+         (m == 1 || (ld * type_size(type)) % 16 == 0) && aligned(norm_w, 16) && aligned(norm_b, 16);
 }
 
 int i8_tensor_map(EncodeTiledFn enc, CUtensorMap* map, const int8_t* base, int rows, int k, int box_rows) {
@@ -2284,17 +2303,8 @@ int launch_i8_tiles(DeviceState* ds, const I8Params& p, cudaStream_t st) {
 }
 
 int launch_i8(DeviceState* ds, const I8Params& p, int y_type, cudaStream_t st) {
-  if (p.m > 8)
-    return with_type(y_type, [&](auto t) { return launch_i8_tiles<decltype(t)>(ds, p, st); });
-  const cudaError_t e = with_type(y_type, [&](auto t) {
-    using T = decltype(t);
-    return p.m <= 1   ? launch_i8_gemv<T, 1>(p, ds->sms, st)
-           : p.m <= 2 ? launch_i8_gemv<T, 2>(p, ds->sms, st)
-           : p.m <= 4 ? launch_i8_gemv<T, 4>(p, ds->sms, st)
-                      : launch_i8_gemv<T, 8>(p, ds->sms, st);
-  });
-  if (e != cudaSuccess) return to_code(e);
-  return to_code(cudaGetLastError());
+  if (p.m <= kI8GemvMaxM) return launch_i8_few<false, float, false>(ds, p, I8Tokens{}, y_type, st);
+  return with_type(y_type, [&](auto t) { return launch_i8_tiles<decltype(t)>(ds, p, st); });
 }
 
 I8Params i8_params(DeviceState* ds, const int8_t* w, const float* w_scale, const int8_t* x, const float* x_scale,
@@ -2394,6 +2404,16 @@ extern "C" int pq8_linear_i8(const int8_t* w, const float* w_scale, const void* 
     return rc;
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
+  if (i8_fused(x, x_type, ld, norm_w, norm_b, m, k)) {
+    const I8Tokens tokens{x, ld, norm_w, norm_b, kNormEps64, x_type};
+    const I8Params p = i8_params(ds, w, w_scale, nullptr, nullptr, y, bias, resid, m, n, k, epilogue, alpha);
+    return with_type(x_type, [&](auto t) {
+      using T = decltype(t);
+      cudaStream_t st = static_cast<cudaStream_t>(stream);
+      return norm_w != nullptr ? launch_i8_few<true, T, true>(ds, p, tokens, y_type, st)
+                               : launch_i8_few<true, T, false>(ds, p, tokens, y_type, st);
+    });
+  }
   if ((rc = quantize_rows(x, x_type, ld, norm_w, norm_b, q, scale, m, k, stream))) return rc;
   return launch_i8(ds, i8_params(ds, w, w_scale, q, scale, y, bias, resid, m, n, k, epilogue, alpha), y_type,
                    static_cast<cudaStream_t>(stream));

@@ -33,48 +33,112 @@ __device__ __forceinline__ float i8_scaled(int acc, float s, float t, float b) {
 }
 
 // ---------------------------------------------------------------------------
-// A few tokens (m <= 8 per pass): the weights are read once, 16 bytes per lane, by
-// dp4a; HBM-bound. A warp takes R channels over the whole of K, a lane every
-// 32nd 16-byte chunk; the lanes' sums meet in one reduction per output.
+// A few tokens (m <= 8): the weights are read once, 16 bytes per lane, by
+// dp4a; latency- and HBM-bound. A warp takes R channels over the whole of K, a
+// lane every 32nd 16-byte chunk; the lanes' sums meet in one reduction per
+// output. With FUSED the tokens arrive in floating point and every CTA
+// quantises them for itself into shared memory (the same few KB from L2 for
+// all of them), which saves the launch and the round trip of a pass of its own.
 constexpr int kI8GemvThreads = 256;
+constexpr int kI8GemvMaxM = 8;
 
-template <typename T, int M, int R>
-__global__ void __launch_bounds__(kI8GemvThreads) i8_gemv_kernel(const I8Params p) {
-  griddep_wait();
-  griddep_launch();
+// Tokens in floating point, for the FUSED form.
+struct I8Tokens {
+  const void* x;
+  long long ld;
+  const float* norm_w;  // LayerNorm first, or NULL
+  const float* norm_b;
+  double eps;
+  int type;
+};
+
+// One value of type `type` (PQ8_TYPE_*) at element `i` of p.
+__device__ __forceinline__ float load_as_f32(const void* p, int type, size_t i) {
+  return type == PQ8_TYPE_F32   ? static_cast<const float*>(p)[i]
+         : type == PQ8_TYPE_F16 ? __half2float(static_cast<const __half*>(p)[i])
+                                : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_from_f32(void* p, int type, size_t i, float v) {
+  if (type == PQ8_TYPE_F32) static_cast<float*>(p)[i] = v;
+  else if (type == PQ8_TYPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// FUSED: tokens of type T, after a LayerNorm with NORM. One token is quantised by
+// the whole CTA (up to 8192 columns), several by a warp each (up to 1024).
+template <int M, int R, bool FUSED, typename T, bool NORM>
+__global__ void __launch_bounds__(kI8GemvThreads, 2) i8_gemv_kernel(const I8Params p, const I8Tokens tokens, int y_type) {
+  extern __shared__ int4 q_smem[];  // FUSED: [m][k] int8
+  __shared__ float scale_smem[M];
+  constexpr int kWarps = kI8GemvThreads / 32, kTeam = M == 1 ? kWarps : 1;
+  __shared__ double team_smem[2 * kTeam];
+  __shared__ float top_smem[kWarps];
   const int lane = threadIdx.x & 31;
-  const int unit = static_cast<int>(blockIdx.x) * (kI8GemvThreads / 32) + (threadIdx.x >> 5);
+  const int unit = static_cast<int>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   const bool glu = p.epi == PQ8_EPI_GLU;
   const int half = p.n >> 1;
   // channel of local row r: consecutive ones, or for GLU the pairs (j, j + n / 2)
   constexpr int P = R > 1 ? R / 2 : 1;
   const int j0 = unit * (glu ? P : R);
-  if (j0 >= p.out_cols) return;
   auto channel = [&](int r) { return glu ? (r < P ? j0 + r : half + j0 + r - P) : j0 + r; };
   auto valid = [&](int r) { return glu ? j0 + r % P < half : j0 + r < p.n; };
   const int chunks = p.k >> 4;
-  for (int m0 = static_cast<int>(blockIdx.y) * M; m0 < p.m; m0 += static_cast<int>(gridDim.y) * M) {
+  const int4* wrow[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    wrow[r] = reinterpret_cast<const int4*>(p.w + static_cast<size_t>(valid(r) ? channel(r) : 0) * p.k);
+  griddep_wait();
+  griddep_launch();
+  // The first weights are on their way while the tokens are quantised.
+  constexpr int kAhead = 2;
+  int4 ahead[kAhead][R];
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      ahead[a][r] = lane + 32 * a < chunks ? __ldg(wrow[r] + lane + 32 * a) : make_int4(0, 0, 0, 0);
+  if constexpr (FUSED) {
+    int8_t* q = reinterpret_cast<int8_t*>(q_smem);
+    std::conditional_t<NORM, LayerNormSource<T, true>, PlainSource<T, true>> src;
+    if constexpr (NORM) {
+      src.w = tokens.norm_w;
+      src.b = tokens.norm_b;
+      src.eps = tokens.eps;
+      src.inv_width = 1.0 / p.k;
+      src.top_b = cta_max_abs(tokens.norm_b, p.k, top_smem);
+    }
+    const RowTeam<kTeam> team{team_smem};
+    const int r = kTeam > 1 ? 0 : threadIdx.x >> 5;
+    if (r < p.m) {
+      src.x = static_cast<const T*>(tokens.x) + r * tokens.ld;
+      const float s = quantize_row<32 / kChunk<T>, kTeam>(src, p.k, q + r * p.k, team);
+      if (team.index() == 0) scale_smem[r] = s;
+    }
+    __syncthreads();
+  }
+  if (j0 >= p.out_cols) return;
+  // lane i finishes the outputs of token i; what it needs besides the sums
+  const int row = lane < M ? min(lane, p.m - 1) : 0;
+  const float s = FUSED ? scale_smem[row] : p.x_scale[row];
+  float t[R], b[R], res[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = valid(r) ? channel(r) : 0;
+    t[r] = p.w_scale[j];
+    b[r] = p.bias ? p.bias[j] : 0.0f;
+    res[r] = p.epi == PQ8_EPI_RESIDUAL ? load_as_f32(p.resid, y_type, static_cast<size_t>(row) * p.out_cols + j) : 0.0f;
+  }
   int acc[R][M];
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int i = 0; i < M; ++i) acc[r][i] = 0;
-  const int4* wrow[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-    wrow[r] = reinterpret_cast<const int4*>(p.w + static_cast<size_t>(valid(r) ? channel(r) : 0) * p.k);
-  const int4* xrow[M];
-#pragma unroll
-  for (int i = 0; i < M; ++i)
-    xrow[i] = reinterpret_cast<const int4*>(p.x + static_cast<size_t>(min(m0 + i, p.m - 1)) * p.k);
-#pragma unroll 2
-  for (int c = lane; c < chunks; c += 32) {
-    int4 wv[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) wv[r] = __ldg(wrow[r] + c);
+  auto add = [&](const int4(&wv)[R], int c) {
 #pragma unroll
     for (int i = 0; i < M; ++i) {
-      const int4 xv = __ldg(xrow[i] + c);
+      const int at = min(i, p.m - 1);
+      const int4 xv = FUSED ? q_smem[at * chunks + c]
+                            : __ldg(reinterpret_cast<const int4*>(p.x + static_cast<size_t>(at) * p.k) + c);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         acc[r][i] = __dp4a(wv[r].x, xv.x, acc[r][i]);
@@ -83,8 +147,17 @@ __global__ void __launch_bounds__(kI8GemvThreads) i8_gemv_kernel(const I8Params 
         acc[r][i] = __dp4a(wv[r].w, xv.w, acc[r][i]);
       }
     }
+  };
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a)
+    if (lane + 32 * a < chunks) add(ahead[a], lane + 32 * a);
+#pragma unroll 2
+  for (int c = lane + 32 * kAhead; c < chunks; c += 32) {
+    int4 wv[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) wv[r] = __ldg(wrow[r] + c);
+    add(wv, c);
   }
-  // every lane gets every sum; lane i keeps the outputs of token i
   int mine[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) mine[r] = 0;
@@ -95,30 +168,21 @@ __global__ void __launch_bounds__(kI8GemvThreads) i8_gemv_kernel(const I8Params 
       const int sum = __reduce_add_sync(0xffffffffu, acc[r][i]);
       if (lane == i) mine[r] = sum;
     }
-  const int row = m0 + lane;
-  if (lane >= M || row >= p.m) continue;
-  const float s = p.x_scale[row];
+  if (lane >= M || lane >= p.m) return;
   float z[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int j = valid(r) ? channel(r) : 0;
-    z[r] = i8_scaled(mine[r], s, p.w_scale[j], p.bias ? p.bias[j] : 0.0f);
-  }
-  T* y = static_cast<T*>(p.y) + static_cast<size_t>(row) * p.out_cols;
-  const T* res = static_cast<const T*>(p.resid) + static_cast<size_t>(row) * p.out_cols;
+  for (int r = 0; r < R; ++r) z[r] = i8_scaled(mine[r], s, t[r], b[r]);
+  const size_t y0 = static_cast<size_t>(row) * p.out_cols + j0;
   if (glu) {
 #pragma unroll
     for (int r = 0; r < P; ++r)
-      if (valid(r)) y[j0 + r] = from_f32<T>(z[r] / (1.0f + expf(-z[R > 1 ? r + P : 0])));
+      if (valid(r)) store_from_f32(p.y, y_type, y0 + r, z[r] / (1.0f + expf(-z[R > 1 ? r + P : 0])));
   } else {
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (valid(r)) {
-        float v = act_f32(z[r], p.epi);
-        if (p.epi == PQ8_EPI_RESIDUAL) v = fmaf(p.alpha, z[r], to_f32(res[j0 + r]));
-        y[j0 + r] = from_f32<T>(v);
-      }
-  }
+      if (valid(r))
+        store_from_f32(p.y, y_type, y0 + r,
+                       p.epi == PQ8_EPI_RESIDUAL ? fmaf(p.alpha, z[r], res[r]) : act_f32(z[r], p.epi));
   }
 }
 
