@@ -513,7 +513,9 @@ PQ8_API int pq8_gemm_i8(const int8_t* w, const float* w_scale, const int8_t* x, 
 /* pq8_quantize_rows (norm_w, norm_b NULL) or pq8_layer_norm_quantize, then
  * pq8_gemm_i8: the linear on tokens in floating point. The
  * quantised tokens live in the workspace (16-byte aligned, no
- * initialisation): calls that may overlap on the GPU need one each. */
+ * initialisation): calls that may overlap on the GPU need one each. One token
+ * of k <= 8192, or up to 8 of k <= 1024, whose rows and norm parameters start
+ * on 16-byte boundaries, take one launch and no workspace (NULL). */
 PQ8_API int pq8_linear_i8_workspace_size(int m, int k, size_t* bytes);
 PQ8_API int pq8_linear_i8(const int8_t* w, const float* w_scale, const void* x, int x_type, long long ld,
                           const float* norm_w, const float* norm_b, void* y, int y_type, const float* bias,
@@ -534,9 +536,12 @@ PQ8_API int pq8_linear_i8(const int8_t* w, const float* w_scale, const void* x, 
  * Sums are FP64, in a fixed order. channels at most 16384, groups at most
  * 4096, rows at most 2^30. y must not overlap x. PQ8_FLAG_OUT_TF32 (type F32)
  * rounds y for a following pq8_gemm. The workspace (16-byte aligned, no
- * initialisation) is per call in flight. No counterpart in the reference,
+ * initialisation) is per call in flight; where its size is 0 it may be NULL.
+ * quantize: 1 for pq8_group_norm_quantize; aligned16: whether x and y (x, w
+ * and b with quantize) start on 16-byte boundaries. No counterpart in the reference,
  * whose conv module has BatchNorm (reference.py:60-63). */
-PQ8_API int pq8_group_norm_workspace_size(int rows, int windows, int channels, int groups, size_t* bytes);
+PQ8_API int pq8_group_norm_workspace_size(int type, int rows, int windows, int channels, int groups, int quantize,
+                                          int aligned16, size_t* bytes);
 PQ8_API int pq8_group_norm(const void* x, int type, const float* w, const float* b, void* y, int rows, int windows,
                            const int* offsets, int channels, int groups, double eps, int activation, int flags,
                            void* workspace, size_t workspace_bytes, void* stream);

@@ -2109,20 +2109,43 @@ bool resid_ok(const void* y, const void* resid, size_t bytes) {
   return y == resid || !overlap(y, bytes, resid, bytes);
 }
 
+// Lets `kernel` use `bytes` of dynamic shared memory, once per device (`done`:
+// one flag per device, of this kernel alone).
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes, bool* done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (done[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  done[dev] = e == cudaSuccess;
+  return e;
+}
+
 size_t rows_bytes(long long rows, long long ld, int width, int size) {
   return static_cast<size_t>((rows - 1) * ld + width) * size;
 }
 
-int check_rows_args(const void* x, int type, long long ld, const float* w, const float* b, const int8_t* q,
-                    const float* scale, int rows, int width) {
+int check_token_args(const void* x, int type, long long ld, const float* w, const float* b, int rows, int width) {
   if (rows < 0 || width <= 0 || width % 16 || width > kI8MaxK) return PQ8_ERR_UNSUPPORTED_SHAPE;
   const int size = type_size(type);
   if (size == 0 || (w == nullptr) != (b == nullptr)) return PQ8_ERR_INVALID_ARGUMENT;
   if (rows == 0) return PQ8_OK;
-  if (x == nullptr || q == nullptr || scale == nullptr || ld < width) return PQ8_ERR_INVALID_ARGUMENT;
-  if (ld > (1LL << 40)) return PQ8_ERR_UNSUPPORTED_SHAPE;
-  if (!aligned(x, size) || !aligned(q, 16) || !aligned(scale, 4) || !aligned(w, 4) || !aligned(b, 4))
-    return PQ8_ERR_MISALIGNED;
+  if (x == nullptr || ld < width) return PQ8_ERR_INVALID_ARGUMENT;
+  if (ld > (1LL << 31)) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  if (!aligned(x, size) || !aligned(w, 4) || !aligned(b, 4)) return PQ8_ERR_MISALIGNED;
+  return PQ8_OK;
+}
+
+int check_rows_args(const void* x, int type, long long ld, const float* w, const float* b, const int8_t* q,
+                    const float* scale, int rows, int width) {
+  const int rc = check_token_args(x, type, ld, w, b, rows, width);
+  if (rc || rows == 0) return rc;
+  if (q == nullptr || scale == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  if (!aligned(q, 16) || !aligned(scale, 4)) return PQ8_ERR_MISALIGNED;
+  const int size = type_size(type);
   const size_t nx = rows_bytes(rows, ld, width, size);
   if (overlap(x, nx, q, static_cast<size_t>(rows) * width) || overlap(x, nx, scale, static_cast<size_t>(rows) * 4))
     return PQ8_ERR_INVALID_ARGUMENT;
@@ -2249,18 +2272,9 @@ int launch_i8_gemm(DeviceState* ds, const I8Params& p, int splits, cudaStream_t 
   const long long slots = ds->sms / per;
   if (splits > 1 && tiles > slots) return PQ8_ERR_INVALID_ARGUMENT;
   auto kernel = i8_gemm_kernel<T, BN, PAIR, STAGES>;
-  static bool attr_set[kMaxDevices];  // guarded by g_mutex, one per kernel
-  {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return to_code(e);
-    std::lock_guard<std::mutex> lock(g_mutex);
-    if (!attr_set[dev]) {
-      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
-      if (e != cudaSuccess) return to_code(e);
-      attr_set[dev] = true;
-    }
-  }
+  static bool attr_set[kMaxDevices];
+  const cudaError_t ea = allow_smem(kernel, C::kSmemBytes, attr_set);
+  if (ea != cudaSuccess) return to_code(ea);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min(tiles, slots) * per));
   cfg.blockDim = dim3(C::kThreads);
@@ -2394,17 +2408,21 @@ extern "C" int pq8_linear_i8(const int8_t* w, const float* w_scale, const void* 
   int rc = check_i8_args(w, w_scale, y, y_type, resid, m, n, k, epilogue);
   if (rc) return rc;
   const I8Workspace ws = plan_linear_i8(m, k);
-  if (m > 0 && (workspace == nullptr || workspace_bytes < ws.total)) return PQ8_ERR_WORKSPACE;
+  const bool fused = i8_fused(x, x_type, ld, norm_w, norm_b, m, k);
   if (!aligned(workspace, 16) || !aligned(bias, 4)) return PQ8_ERR_MISALIGNED;
-  int8_t* q = static_cast<int8_t*>(workspace);
-  float* scale = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + ws.scale);
-  if ((rc = check_rows_args(x, x_type, ld, norm_w, norm_b, q, scale, m, k)) || m == 0) return rc;
-  if ((rc = check_i8_overlap(w, w_scale, x, rows_bytes(m, ld, k, type_size(x_type)), scale, y, y_type, bias, resid, m,
-                             n, k, epilogue)))
-    return rc;
+  if ((rc = check_token_args(x, x_type, ld, norm_w, norm_b, m, k)) || m == 0) return rc;
+  if (!fused && (workspace == nullptr || workspace_bytes < ws.total)) return PQ8_ERR_WORKSPACE;
+  int8_t* q = fused ? nullptr : static_cast<int8_t*>(workspace);
+  float* scale = fused ? nullptr : reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + ws.scale);
+  const size_t x_bytes = rows_bytes(m, ld, k, type_size(x_type));
+  if (!fused && overlap(x, x_bytes, workspace, ws.total)) return PQ8_ERR_INVALID_ARGUMENT;
+  if ((rc = check_i8_overlap(w, w_scale, x, x_bytes, nullptr, y, y_type, bias, resid, m, n, k, epilogue))) return rc;
+  if (!fused && overlap(y, static_cast<size_t>(m) * (epilogue == PQ8_EPI_GLU ? n / 2 : n) * type_size(y_type),
+                        workspace, ws.total))
+    return PQ8_ERR_INVALID_ARGUMENT;
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
-  if (i8_fused(x, x_type, ld, norm_w, norm_b, m, k)) {
+  if (fused) {
     const I8Tokens tokens{x, ld, norm_w, norm_b, kNormEps64, x_type};
     const I8Params p = i8_params(ds, w, w_scale, nullptr, nullptr, y, bias, resid, m, n, k, epilogue, alpha);
     return with_type(x_type, [&](auto t) {
@@ -2424,48 +2442,100 @@ namespace pq8 {
 namespace {
 
 struct GroupNormPlan {
-  int chunks, slab, slabs, grid_y;
-  size_t total;
+  int units;          // NormUnits
+  int slab, slabs;    // whole groups per CTA
+  int parts;          // one launch: CTAs of a window's cluster; 0: two launches
+  int hold;           // one launch: rows a CTA holds
+  size_t smem;        // one launch
+  int chunks, apply;  // two launches: row chunks of the sums, and of the second launch
+  size_t total;       // workspace
 };
 
-// Row chunks per window so that windows x slabs x chunks fill the SMs a few
-// times, with at least 8 rows a chunk.
-GroupNormPlan plan_group_norm(int rows, int windows, int channels, int groups) {
+constexpr size_t kNormMaxSmem = size_t(200) << 10;
+
+// `vec`: 16-byte loads fit the addresses. The same for every device, so that the
+// workspace can be sized without one.
+GroupNormPlan plan_group_norm(int size, bool vec, int rows, int windows, int channels, int groups, bool quantize) {
+  constexpr int sms = 148;
   GroupNormPlan g{};
-  const int cg = channels / groups;
-  g.slab = std::max(1, std::min(groups, kNormThreads / cg));
+  const int cg = channels / groups, E = 16 / size;
+  g.units = kScalar;
+  int least = 1;  // groups whose columns are whole units
+  if (vec && channels % E == 0) {
+    if (cg % E == 0) {
+      g.units = kWhole;
+    } else if (cg > E) {
+      while (least * cg % E) ++least;
+      if (least * cg / E <= kNormThreads) g.units = kStraddle;
+      else least = 1;
+    }
+  }
+  const int unit = g.units == kScalar ? 1 : E;
+  // columns of a row that a CTA reads: at least 128 bytes, so that whole
+  // sectors are used, within the CTA's threads
+  g.slab = least;
+  while (g.slab * cg * size < 128 && g.slab + least <= groups && (g.slab + least) * cg / unit <= kNormThreads)
+    g.slab += least;
   g.slabs = (groups + g.slab - 1) / g.slab;
-  const int per_window = std::max(1, rows / std::max(1, windows));
-  const long long units = static_cast<long long>(windows) * g.slabs;
-  g.chunks = static_cast<int>(std::max<long long>(1, std::min<long long>({64, (per_window + 7) / 8, 1184 / units})));
-  g.grid_y = std::min(windows, 65535);
+  const long long units = static_cast<long long>(std::max(windows, 1)) * g.slabs;
+  const int t = std::max(1, (rows + std::max(windows, 1) - 1) / std::max(windows, 1));
+  const size_t row_bytes = static_cast<size_t>(g.slab) * cg * size;
+  if (!quantize && g.units != kScalar && windows <= 65535) {
+    // One launch: the smallest cluster that holds an average window at four
+    // CTAs an SM, and that gives every SM a CTA; at most 8 CTAs.
+    int parts = 1;
+    while (parts < 8 && ((t + parts - 1) / parts * row_bytes > (48 << 10) ||
+                         (units * parts < sms && t / (2 * parts) >= 16)))
+      parts *= 2;
+    const int per = (t + parts - 1) / parts;
+    const size_t tables = static_cast<size_t>(g.slab) * (sizeof(GroupSum) + sizeof(GroupStat));
+    if (per * row_bytes + tables <= kNormMaxSmem) {
+      g.parts = parts;
+      g.hold = per;
+      g.smem = per * row_bytes + tables;
+      return g;
+    }
+  }
+  // Two launches: row chunks that fill the SMs a few times, eight rows at least.
+  const long long fill = std::max<long long>(1, 8LL * sms / units);
+  g.chunks = static_cast<int>(std::min<long long>({64, (t + 7) / 8, fill}));
+  g.apply = static_cast<int>(std::min<long long>((t + 7) / 8, quantize ? std::max<long long>(1, 6LL * sms / std::max(windows, 1)) : fill));
   g.total = round256(sizeof(GroupSum) * static_cast<size_t>(windows) * g.chunks * groups);
   return g;
 }
 
-int check_group_norm(const void* x, int type, const float* w, const float* b, const void* y, size_t y_bytes, int rows,
-                     int windows, const int* offsets, int channels, int groups, double eps, int act, void* workspace,
-                     size_t workspace_bytes) {
+int check_group_norm_shape(int type, int rows, int windows, int channels, int groups) {
   if (rows < 0 || rows > (1 << 30) || windows < 0 || windows > (1 << 24) || channels < 1 || channels > 16384 ||
       groups < 1 || groups > 4096 || channels % groups)
     return PQ8_ERR_UNSUPPORTED_SHAPE;
+  return type_size(type) ? PQ8_OK : PQ8_ERR_INVALID_ARGUMENT;
+}
+
+int check_group_norm(const void* x, int type, const float* w, const float* b, const void* y, size_t y_bytes, int rows,
+                     int windows, const int* offsets, int channels, int groups, double eps, int act,
+                     const void* workspace) {
   if (offsets == nullptr && windows > 0 && rows % windows) return PQ8_ERR_UNSUPPORTED_SHAPE;
   const int size = type_size(type);
-  if (size == 0 || !(eps > 0.0) || !(eps < 1e30) ||
-      (act != PQ8_EPI_NONE && act != PQ8_EPI_RELU && act != PQ8_EPI_SILU))
+  if (!(eps > 0.0) || !(eps < 1e30) || (act != PQ8_EPI_NONE && act != PQ8_EPI_RELU && act != PQ8_EPI_SILU))
     return PQ8_ERR_INVALID_ARGUMENT;
   if (rows == 0 || windows == 0) return PQ8_OK;
   if (x == nullptr || w == nullptr || b == nullptr || y == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
   if (!aligned(x, size) || !aligned(w, 4) || !aligned(b, 4) || !aligned(offsets, 4) || !aligned(workspace, 16))
     return PQ8_ERR_MISALIGNED;
-  if (overlap(y, y_bytes, x, static_cast<size_t>(rows) * channels * size) ||
-      overlap(y, y_bytes, w, static_cast<size_t>(channels) * 4) ||
+  const size_t x_bytes = static_cast<size_t>(rows) * channels * size;
+  if (overlap(y, y_bytes, x, x_bytes) || overlap(y, y_bytes, w, static_cast<size_t>(channels) * 4) ||
       overlap(y, y_bytes, b, static_cast<size_t>(channels) * 4) ||
       overlap(y, y_bytes, offsets, (static_cast<size_t>(windows) + 1) * 4))
     return PQ8_ERR_INVALID_ARGUMENT;
-  const GroupNormPlan g = plan_group_norm(rows, windows, channels, groups);
-  if (workspace == nullptr || workspace_bytes < g.total) return PQ8_ERR_WORKSPACE;
   return PQ8_OK;
+}
+
+// The workspace of the two-launch form: present, and no part of x or y.
+int check_norm_workspace(const GroupNormPlan& g, const void* ws, size_t ws_bytes, const void* x, size_t x_bytes,
+                         const void* y, size_t y_bytes) {
+  if (g.total == 0) return PQ8_OK;
+  if (ws == nullptr || ws_bytes < g.total) return PQ8_ERR_WORKSPACE;
+  return overlap(ws, g.total, x, x_bytes) || overlap(ws, g.total, y, y_bytes) ? PQ8_ERR_INVALID_ARGUMENT : PQ8_OK;
 }
 
 GroupNormParams group_norm_params(const GroupNormPlan& g, const void* x, const float* w, const float* b, int rows,
@@ -2483,57 +2553,97 @@ GroupNormParams group_norm_params(const GroupNormPlan& g, const void* x, const f
   p.eps = eps;
   p.chunks = g.chunks;
   p.slab = g.slab;
+  p.hold = g.hold;
   return p;
 }
 
+// f(the plan's unit form as a type)
+template <int V>
+struct UnitsTag {
+  static constexpr int value = V;
+};
+template <typename F>
+auto with_units(int units, F&& f) {
+  return units == kWhole ? f(UnitsTag<kWhole>{}) : units == kStraddle ? f(UnitsTag<kStraddle>{}) : f(UnitsTag<kScalar>{});
+}
+
+template <typename T, int UNITS>
+cudaError_t launch_group_norm_one(const GroupNormPlan& g, const GroupNormParams& p, T* y, cudaStream_t st) {
+  auto kernel = group_norm_kernel<T, UNITS>;
+  static bool attr_set[kMaxDevices];
+  const cudaError_t ea = allow_smem(kernel, static_cast<int>(kNormMaxSmem), attr_set);
+  if (ea != cudaSuccess) return ea;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(g.parts, p.windows, g.slabs);
+  cfg.blockDim = dim3(kNormThreads);
+  cfg.dynamicSmemBytes = g.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = g.parts;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g.parts > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p, y);
+}
+
 template <typename T>
-cudaError_t launch_group_stats(const GroupNormPlan& g, const GroupNormParams& p, bool vec, GroupSum* partial,
-                               cudaStream_t st) {
-  const dim3 grid(g.chunks, g.grid_y, g.slabs);
-  return vec ? launch_pdl(group_stats_kernel<T, true>, grid, dim3(kNormThreads), 0, st, p, partial)
-             : launch_pdl(group_stats_kernel<T, false>, grid, dim3(kNormThreads), 0, st, p, partial);
+cudaError_t launch_group_stats(const GroupNormPlan& g, const GroupNormParams& p, GroupSum* partial, cudaStream_t st) {
+  const dim3 grid(g.chunks, std::min(p.windows, 65535), g.slabs);
+  return with_units(g.units, [&](auto u) {
+    return launch_pdl(group_stats_kernel<T, decltype(u)::value>, grid, dim3(kNormThreads), 0, st, p, partial);
+  });
 }
 
 }  // namespace
 }  // namespace pq8
 
-extern "C" int pq8_group_norm_workspace_size(int rows, int windows, int channels, int groups, size_t* bytes) {
+extern "C" int pq8_group_norm_workspace_size(int type, int rows, int windows, int channels, int groups, int quantize,
+                                             int aligned16, size_t* bytes) {
   if (bytes == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
-  if (rows < 0 || rows > (1 << 30) || windows < 0 || windows > (1 << 24) || channels < 1 || channels > 16384 ||
-      groups < 1 || groups > 4096 || channels % groups)
-    return PQ8_ERR_UNSUPPORTED_SHAPE;
-  *bytes = plan_group_norm(rows, windows, channels, groups).total;
+  const int rc = check_group_norm_shape(type, rows, windows, channels, groups);
+  if (rc) return rc;
+  *bytes = 0;
+  if (rows > 0 && windows > 0)
+    *bytes = plan_group_norm(type_size(type), aligned16 != 0, rows, windows, channels, groups, quantize != 0).total;
   return PQ8_OK;
 }
 
 extern "C" int pq8_group_norm(const void* x, int type, const float* w, const float* b, void* y, int rows, int windows,
                               const int* offsets, int channels, int groups, double eps, int activation, int flags,
                               void* workspace, size_t workspace_bytes, void* stream) {
-  if (type_size(type) == 0 || (flags & ~PQ8_FLAG_OUT_TF32) || ((flags & PQ8_FLAG_OUT_TF32) && type != PQ8_TYPE_F32))
+  int rc = check_group_norm_shape(type, rows, windows, channels, groups);
+  if (rc) return rc;
+  if ((flags & ~PQ8_FLAG_OUT_TF32) || ((flags & PQ8_FLAG_OUT_TF32) && type != PQ8_TYPE_F32))
     return PQ8_ERR_INVALID_ARGUMENT;
-  const size_t bytes = static_cast<size_t>(std::max(rows, 0)) * std::max(channels, 0) * type_size(type);
-  int rc = check_group_norm(x, type, w, b, y, bytes, rows, windows, offsets, channels, groups, eps, activation,
-                            workspace, workspace_bytes);
+  const size_t bytes = static_cast<size_t>(rows) * channels * type_size(type);
+  rc = check_group_norm(x, type, w, b, y, bytes, rows, windows, offsets, channels, groups, eps, activation, workspace);
   if (rc || rows == 0 || windows == 0) return rc;
   if (!aligned(y, type_size(type))) return PQ8_ERR_MISALIGNED;
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
+  const GroupNormPlan g = plan_group_norm(type_size(type), aligned(x, 16) && aligned(y, 16), rows, windows, channels,
+                                          groups, false);
+  if ((rc = check_norm_workspace(g, workspace, workspace_bytes, x, bytes, y, bytes))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const GroupNormPlan g = plan_group_norm(rows, windows, channels, groups);
   const cudaError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
     GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
     p.round_out = (flags & PQ8_FLAG_OUT_TF32) ? 1 : 0;
-    const bool vec = (channels / groups) % kChunk<T> == 0 && aligned(x, 16) && aligned(y, 16);
+    if (g.parts > 0)
+      return g.units == kWhole ? launch_group_norm_one<T, kWhole>(g, p, static_cast<T*>(y), st)
+                               : launch_group_norm_one<T, kStraddle>(g, p, static_cast<T*>(y), st);
     GroupSum* partial = static_cast<GroupSum*>(workspace);
-    cudaError_t err = launch_group_stats<T>(g, p, vec, partial, st);
+    const cudaError_t err = launch_group_stats<T>(g, p, partial, st);
     if (err != cudaSuccess) return err;
-    const dim3 grid(g.chunks, g.grid_y, g.slabs);
-    const size_t smem = sizeof(GroupStat) * g.slab;
-    return vec ? launch_pdl(group_apply_kernel<T, true>, grid, dim3(kNormThreads), smem, st, p,
-                            static_cast<const GroupSum*>(partial), static_cast<T*>(y))
-               : launch_pdl(group_apply_kernel<T, false>, grid, dim3(kNormThreads), smem, st, p,
-                            static_cast<const GroupSum*>(partial), static_cast<T*>(y));
+    const dim3 grid(g.apply, std::min(windows, 65535), g.slabs);
+    return with_units(g.units, [&](auto u) {
+      return launch_pdl(group_apply_kernel<T, decltype(u)::value>, grid, dim3(kNormThreads),
+                        sizeof(GroupStat) * g.slab, st, p, static_cast<const GroupSum*>(partial), static_cast<T*>(y));
+    });
   });
   if (e != cudaSuccess) return to_code(e);
   return to_code(cudaGetLastError());
@@ -2543,35 +2653,37 @@ extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, 
                                        float* scale, int rows, int windows, const int* offsets, int channels,
                                        int groups, double eps, int activation, void* workspace,
                                        size_t workspace_bytes, void* stream) {
+  int rc = check_group_norm_shape(type, rows, windows, channels, groups);
+  if (rc) return rc;
   if (channels % 16) return PQ8_ERR_UNSUPPORTED_SHAPE;
-  const size_t bytes = static_cast<size_t>(std::max(rows, 0)) * std::max(channels, 0);
-  int rc = check_group_norm(x, type, w, b, q, bytes, rows, windows, offsets, channels, groups, eps, activation,
-                            workspace, workspace_bytes);
+  const size_t q_bytes = static_cast<size_t>(rows) * channels, x_bytes = q_bytes * type_size(type);
+  rc = check_group_norm(x, type, w, b, q, q_bytes, rows, windows, offsets, channels, groups, eps, activation,
+                        workspace);
   if (rc || rows == 0 || windows == 0) return rc;
-  if (scale == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  if (scale == nullptr || overlap(scale, static_cast<size_t>(rows) * 4, x, x_bytes)) return PQ8_ERR_INVALID_ARGUMENT;
   if (!aligned(q, 16) || !aligned(scale, 4)) return PQ8_ERR_MISALIGNED;
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
+  const bool vec = aligned(x, 16) && aligned(w, 16) && aligned(b, 16);
+  const GroupNormPlan g = plan_group_norm(type_size(type), vec, rows, windows, channels, groups, true);
+  if ((rc = check_norm_workspace(g, workspace, workspace_bytes, x, x_bytes, q, q_bytes))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const GroupNormPlan g = plan_group_norm(rows, windows, channels, groups);
   const cudaError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
-    GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
-    const bool vec = aligned(x, 16) && aligned(w, 16) && aligned(b, 16);
+    const GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
     GroupSum* partial = static_cast<GroupSum*>(workspace);
-    cudaError_t err = launch_group_stats<T>(g, p, vec && (channels / groups) % kChunk<T> == 0, partial, st);
+    cudaError_t err = launch_group_stats<T>(g, p, partial, st);
     if (err != cudaSuccess) return err;
-    const dim3 grid(g.chunks * g.slabs, g.grid_y);
+    const dim3 grid(g.apply, std::min(windows, 65535));
     const size_t smem = (sizeof(GroupStat) + sizeof(float4)) * groups;
     constexpr int C = 32 / kChunk<T>;
     auto kernel = !vec               ? group_quantize_kernel<T, 0, 8, false>
                   : channels <= 1024 ? group_quantize_kernel<T, C, 1, true>
                   : channels <= 8192 ? group_quantize_kernel<T, C, 8, true>
                                      : group_quantize_kernel<T, 0, 8, true>;
-    if (smem > 48 * 1024 - 256) {
-      err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-      if (err != cudaSuccess) return err;
-    }
+    static bool attr_set[4][kMaxDevices];
+    const int which = !vec ? 0 : channels <= 1024 ? 1 : channels <= 8192 ? 2 : 3;
+    if ((err = allow_smem(kernel, 4096 * 32, attr_set[which])) != cudaSuccess) return err;
     return launch_pdl(kernel, grid, dim3(kRowThreads), smem, st, p, static_cast<const GroupSum*>(partial), q, scale);
   });
   if (e != cudaSuccess) return to_code(e);

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kI8GemvThreads, 2) i8_gemv_kernel(const I8Para
   if (glu) {
 #pragma unroll
     for (int r = 0; r < P; ++r)
-      if (valid(r)) store_from_f32(p.y, y_type, y0 + r, z[r] / (1.0f + expf(-z[R > 1 ? r + P : 0])));
+      if (valid(r)) store_from_f32(p.y, y_type, y0 + r, __fdividef(z[r], 1.0f + __expf(-z[R > 1 ? r + P : 0])));
   } else {
 #pragma unroll
     for (int r = 0; r < R; ++r)

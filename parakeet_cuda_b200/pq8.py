@@ -105,10 +105,19 @@ SIGNATURES = {
     'pq8_gemm_i8': ([_P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _P], _I),
     'pq8_linear_i8_workspace_size': ([_I, _I, C.POINTER(_SZ)], _I),
     'pq8_linear_i8': ([_P, _P, _P, _I, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _P, _SZ, _P], _I),
-    'pq8_group_norm_workspace_size': ([_I, _I, _I, _I, C.POINTER(_SZ)], _I),
+    'pq8_group_norm_workspace_size': ([_I, _I, _I, _I, _I, _I, _I, C.POINTER(_SZ)], _I),
     'pq8_group_norm': ([_P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _D, _I, _I, _P, _SZ, _P], _I),
     'pq8_group_norm_quantize': ([_P, _I, _P, _P, _P, _P, _I, _I, _P, _I, _I, _D, _I, _P, _SZ, _P], _I),
 }
+
+
+def linear_i8_scratch(m: int, k: int, starts: int) -> int:
+    """Workspace bytes of ``pq8_linear_i8``, without a call (the library refuses less than it needs).
+    ``starts``: the bits of every address and row distance that has to be a multiple of 16 for
+    the one-launch form of a few tokens, which needs none."""
+    if m <= 8 and k <= (8192 if m == 1 else 1024) and not starts & 15:
+        return 0
+    return (m * k + 255 & ~255) + (4 * m + 255 & ~255)
 
 
 def header_symbols(path: Path = HEADER):
@@ -184,9 +193,11 @@ class Library:
         self.call('pq8_linear_i8_workspace_size', m, k, C.byref(out))
         return out.value
 
-    def group_norm_workspace_size(self, rows: int, windows: int, channels: int, groups: int) -> int:
+    def group_norm_workspace_size(self, kind: int, rows: int, windows: int, channels: int, groups: int,
+                                  quantize: bool = False, aligned16: bool = True) -> int:
         out = _SZ()
-        self.call('pq8_group_norm_workspace_size', rows, windows, channels, groups, C.byref(out))
+        self.call('pq8_group_norm_workspace_size', kind, rows, windows, channels, groups, quantize, aligned16,
+                  C.byref(out))
         return out.value
 
     def stem_workspace_size(self, windows: int, frames: int) -> int:

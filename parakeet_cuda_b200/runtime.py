@@ -27,6 +27,11 @@ from .pq8 import (EPI_GLU, EPI_NONE, GEMV_MAX_M, LAYOUT_GATES4, LAYOUT_GLU, LAYO
 
 MIB = 1 << 20
 
+# The current stream's handle by device index. torch.cuda.current_stream builds a Stream object
+# around it, which costs as much as a launch.
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 
 def _ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
@@ -53,19 +58,35 @@ class PackedWeight:
 ELEMENT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
 
 
-@dataclass
-class Int8Weight:
-    """Weights for the product in 8-bit integers: ``q`` int8 [n, k] (dense), ``scale`` float32 [n]."""
-    q: torch.Tensor
-    scale: torch.Tensor
+class _Int8Rows:
+    """A dense int8 matrix with a float32 scale per row, checked once when it is made."""
+    __slots__ = ('_q', '_scale', 'n', 'k', 'device', 'q_ptr', 'scale_ptr')
+    q = property(lambda self: self._q)
+    scale = property(lambda self: self._scale)
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor):
+        if q.dtype != torch.int8 or q.dim() != 2 or not q.is_contiguous():
+            raise ValueError(f'q must be a contiguous int8 matrix, got {q.dtype} {tuple(q.shape)}')
+        if scale.dtype != torch.float32 or scale.dim() != 1 or not scale.is_contiguous():
+            raise ValueError(f'scale must be a contiguous float32 vector, got {scale.dtype} {tuple(scale.shape)}')
+        self.n, self.k = q.shape
+        if scale.shape[0] != self.n:
+            raise ValueError(f'{self.n} rows need {self.n} scales, got {scale.shape[0]}')
+        self.device = q.device
+        if scale.device != self.device:
+            raise ValueError(f'q is on {q.device}, scale on {scale.device}')
+        self._q, self._scale, self.q_ptr, self.scale_ptr = q, scale, q.data_ptr(), scale.data_ptr()
 
 
-@dataclass
-class QuantizedRows:
-    """Tokens quantised row by row: ``q`` int8 [rows, width] (dense), ``scale`` float32 [rows];
-    row i stands for ``q[i] * scale[i]``."""
-    q: torch.Tensor
-    scale: torch.Tensor
+class Int8Weight(_Int8Rows):
+    """Weights for the product in 8-bit integers: ``q`` int8 [n, k], ``scale`` float32 [n], one per output channel."""
+    __slots__ = ()
+
+
+class QuantizedRows(_Int8Rows):
+    """Tokens quantised row by row: ``q`` int8 [rows, width], ``scale`` float32 [rows]; row i stands for
+    ``q[i] * scale[i]``."""
+    __slots__ = ()
 
 
 def pack_host(raw, n: int, k: int, layout: int = LAYOUT_ROWS, lib=None) -> np.ndarray:
@@ -201,6 +222,8 @@ class Runtime:
         if not torch.cuda.is_available():
             raise RuntimeError('pq8 needs a CUDA device (B200, sm_100a); no CPU fallback exists')
         self.device = torch.device('cuda', device) if isinstance(device, int) else torch.device(device)
+        if self.device.index is None:
+            self.device = torch.device('cuda', torch.cuda.current_device())
         self.lib = pq8.library()
         with torch.cuda.device(self.device):
             self.workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=self.device)
@@ -291,64 +314,56 @@ class Runtime:
         return out
 
     # -- products in 8-bit integers -------------------------------------------
-    def _check(self, t: torch.Tensor, what: str, dtype=None, shape=None) -> None:
-        """A dense tensor on this device, of ``dtype`` and ``shape`` where given."""
-        if t.device != self.device:
-            raise ValueError(f'{what} is on {t.device}, the runtime on {self.device}')
-        if dtype is not None and t.dtype != dtype:
-            raise ValueError(f'{what} must be {dtype}, got {t.dtype}')
-        if shape is not None and t.shape != shape:
-            raise ValueError(f'{what} must have shape {tuple(shape)}, got {tuple(t.shape)}')
-        if not t.is_contiguous():
-            raise ValueError(f'{what} must be contiguous')
+    # These calls take a few microseconds of GPU time for a few tokens, so the
+    # host path is kept short: each tensor is checked once, and outputs are
+    # allocated by the cheapest call torch has for it.
+    def _check(self, t: torch.Tensor, what: str, dtype, shape) -> int:
+        """Address of a dense tensor of ``dtype`` and ``shape`` on this device."""
+        if t.dtype != dtype or t.shape != shape or t.device != self.device or not t.is_contiguous():
+            raise ValueError(f'{what} must be contiguous {dtype} {tuple(shape)} on {self.device}, got '
+                             f'{"" if t.is_contiguous() else "strided "}{t.dtype} {tuple(t.shape)} on {t.device}')
+        return t.data_ptr()
 
     def _check_rows(self, x: torch.Tensor) -> tuple[int, int, int, int]:
         """(rows, width, row distance, type code) of a matrix whose rows are dense."""
         kind = ELEMENT_TYPES.get(x.dtype)
-        if kind is None:
-            raise ValueError(f'x must be float32, float16 or bfloat16, got {x.dtype}')
-        if x.dim() != 2:
-            raise ValueError(f'x must be a matrix, got {x.dim()} dimensions')
-        if x.device != self.device:
-            raise ValueError(f'x is on {x.device}, the runtime on {self.device}')
+        if kind is None or x.dim() != 2 or x.device != self.device:
+            raise ValueError(f'x must be a float32, float16 or bfloat16 matrix on {self.device}, got {x.dtype} '
+                             f'{tuple(x.shape)} on {x.device}')
         rows, width = x.shape
         ld, step = x.stride()
         if rows <= 1:
             ld = width
-        if step != 1 and width > 1 or ld < width:
+        if (step != 1 and width > 1) or ld < width:
             raise ValueError(f'the rows of x must be dense and apart, got strides {x.stride()}')
         return rows, width, ld, kind
 
-    def _check_norm(self, norm, width: int) -> tuple[int | None, int | None]:
-        if norm is None:
-            return None, None
-        w, b = norm
-        self._check(w, 'the norm weight', torch.float32, (width,))
-        self._check(b, 'the norm bias', torch.float32, (width,))
-        return w.data_ptr(), b.data_ptr()
-
-    def _call(self, name: str, *args) -> None:
+    def _enqueue(self, call: str, *args) -> None:
         """A library call on this device's current stream."""
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        if torch.cuda.current_device() == self.device.index:
-            self.lib.call(name, *args, stream)
+        index = self.device.index
+        args += (_raw_stream(index),)
+        if torch.cuda.current_device() == index:
+            code = getattr(self.lib.lib, call)(*args)
         else:
-            with torch.cuda.device(self.device):
-                self.lib.call(name, *args, stream)
+            with torch.cuda.device(index):
+                code = getattr(self.lib.lib, call)(*args)
+        if code:
+            raise pq8.PQ8Error(call, code, self.lib.error_string(code))
 
     def quantize_rows(self, x: torch.Tensor, norm=None) -> QuantizedRows:
         """``x`` [rows, width] (float32, float16 or bfloat16; rows dense, any row distance) to 8-bit
         integers with one scale per row, ``norm=(weight, bias)`` applying LayerNorm first. The
         integers are those of the exact quotient (ties to even); ``width`` a multiple of 16."""
         rows, width, ld, kind = self._check_rows(x)
-        w, b = self._check_norm(norm, width)
         out = QuantizedRows(torch.empty(rows, width, dtype=torch.int8, device=self.device),
                             torch.empty(rows, dtype=torch.float32, device=self.device))
-        args = (out.q.data_ptr(), out.scale.data_ptr(), rows, width)
         if norm is None:
-            self._call('pq8_quantize_rows', x.data_ptr(), kind, ld, *args)
+            self._enqueue('pq8_quantize_rows', x.data_ptr(), kind, ld, out.q_ptr, out.scale_ptr, rows, width)
         else:
-            self._call('pq8_layer_norm_quantize', x.data_ptr(), kind, ld, w, b, *args)
+            w = self._check(norm[0], 'the norm weight', torch.float32, (width,))
+            b = self._check(norm[1], 'the norm bias', torch.float32, (width,))
+            self._enqueue('pq8_layer_norm_quantize', x.data_ptr(), kind, ld, w, b, out.q_ptr, out.scale_ptr, rows,
+                          width)
         return out
 
     def int8_weight(self, w) -> Int8Weight:
@@ -360,7 +375,7 @@ class Runtime:
             if blocks.numel() != n * k // 32 * 34:
                 raise ValueError(f'expected {n * k // 32 * 34} Q8_0 bytes for [{n}, {k}], got {blocks.numel()}')
             w = torch.empty(n, k, dtype=torch.float32, device=self.device)
-            self._call('pq8_dequant_q8_0', blocks.data_ptr(), w.data_ptr(), n * k)
+            self._enqueue('pq8_dequant_q8_0', blocks.data_ptr(), w.data_ptr(), n * k)
         rows = self.quantize_rows(w)
         return Int8Weight(rows.q, rows.scale)
 
@@ -372,62 +387,63 @@ class Runtime:
         ``norm=(weight, bias)``), or ``QuantizedRows``. Epilogues as ``linear``; ``EPI_GLU`` takes the
         plain rows of ``w`` (gates in the second half). ``out_dtype``: float32 (the default),
         float16 or bfloat16; ``out``, ``resid`` have it. ``out`` may be ``resid``, no other input."""
-        n, k = w.q.shape
-        self._check(w.q, 'the weight', torch.int8)
-        self._check(w.scale, 'the weight scale', torch.float32, (n,))
-        quantized = isinstance(x, QuantizedRows)
+        device = self.device
+        if type(w) is not Int8Weight or w.device != device:
+            raise ValueError(f'the weight must be an Int8Weight on {device}')
+        n, k = w.n, w.k
+        quantized = type(x) is QuantizedRows
         if quantized:
+            rows, width = x.n, x.k
             if norm is not None:
                 raise ValueError('quantised tokens take no norm')
-            rows, width = x.q.shape
-            self._check(x.q, 'x', torch.int8)
-            self._check(x.scale, 'the scale of x', torch.float32, (rows,))
+            if x.device != device:
+                raise ValueError(f'x is on {x.device}, the runtime on {device}')
         else:
             rows, width, ld, kind = self._check_rows(x)
-            norm_w, norm_b = self._check_norm(norm, width)
         if width != k:
             raise ValueError(f'x has {width} columns, weight has {k}')
-        shape = (rows, n // 2 if epilogue == EPI_GLU else n)
+        cols = n // 2 if epilogue == EPI_GLU else n
         if out is None:
-            out = torch.empty(shape, dtype=out_dtype or torch.float32, device=self.device)
+            out = torch.empty(rows, cols, dtype=out_dtype or torch.float32, device=device)
+            y = out.data_ptr()
         else:
-            self._check(out, 'out', out_dtype, shape)
+            y = self._check(out, 'out', out_dtype or out.dtype, (rows, cols))
         y_kind = ELEMENT_TYPES.get(out.dtype)
         if y_kind is None:
             raise ValueError(f'the output must be float32, float16 or bfloat16, got {out.dtype}')
-        if bias is not None:
-            self._check(bias, 'bias', torch.float32, (n,))
-        if resid is not None:
-            self._check(resid, 'resid', out.dtype, shape)
-        # (the tensors stay bound here until the launch: a pointer alone would not keep their memory)
-        bias_ptr, resid_ptr = _ptr(bias), _ptr(resid)
+        b = None if bias is None else self._check(bias, 'bias', torch.float32, (n,))
+        r = None if resid is None else self._check(resid, 'resid', out.dtype, (rows, cols))
         if quantized:
-            self._call('pq8_gemm_i8', w.q.data_ptr(), w.scale.data_ptr(), x.q.data_ptr(), x.scale.data_ptr(),
-                       out.data_ptr(), y_kind, bias_ptr, resid_ptr, rows, n, k, epilogue, float(alpha))
-        else:
-            # scratch of this call alone: calls on other streams and captured graphs have their own
-            need = self.lib.linear_i8_workspace_size(rows, k)
-            scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
-            self._call('pq8_linear_i8', w.q.data_ptr(), w.scale.data_ptr(), x.data_ptr(), kind, ld, norm_w, norm_b,
-                       out.data_ptr(), y_kind, bias_ptr, resid_ptr, rows, n, k, epilogue, float(alpha), scratch.data_ptr(),
-                       need)
+            self._enqueue('pq8_gemm_i8', w.q_ptr, w.scale_ptr, x.q_ptr, x.scale_ptr, y, y_kind, b, r, rows, n, k,
+                          epilogue, alpha)
+            return out
+        g = h = None
+        if norm is not None:
+            g = self._check(norm[0], 'the norm weight', torch.float32, (k,))
+            h = self._check(norm[1], 'the norm bias', torch.float32, (k,))
+        # scratch of this call alone: calls on other streams and captured graphs have their own
+        at = x.data_ptr()
+        need = pq8.linear_i8_scratch(rows, k, at | (0 if rows <= 1 else ld * x.element_size()) | (g or 0) | (h or 0))
+        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        self._enqueue('pq8_linear_i8', w.q_ptr, w.scale_ptr, at, kind, ld, g, h, y, y_kind, b, r, rows, n, k,
+                      epilogue, alpha, _ptr(scratch), need)
         return out
 
     # -- group norm --------------------------------------------------------------
     def _check_group_norm(self, x, weight, bias, windows, offsets):
+        """(rows, channels, type code, addresses of x, weight, bias and offsets)."""
         kind = ELEMENT_TYPES.get(x.dtype)
-        if kind is None:
-            raise ValueError(f'x must be float32, float16 or bfloat16, got {x.dtype}')
-        if x.dim() != 2:
-            raise ValueError(f'x must be a matrix, got {x.dim()} dimensions')
-        self._check(x, 'x')
+        if kind is None or x.dim() != 2:
+            raise ValueError(f'x must be a float32, float16 or bfloat16 matrix, got {x.dtype} {tuple(x.shape)}')
         rows, channels = x.shape
-        self._check_norm((weight, bias), channels)
+        at = (self._check(x, 'x', x.dtype, x.shape), self._check(weight, 'weight', torch.float32, (channels,)),
+              self._check(bias, 'bias', torch.float32, (channels,)))
+        off = None
         if offsets is not None:
-            self._check(offsets, 'offsets', torch.int32, (windows + 1,))
+            off = self._check(offsets, 'offsets', torch.int32, (windows + 1,))
         elif windows < 1 or rows % windows:
             raise ValueError(f'{rows} rows do not make {windows} windows of equal length')
-        return rows, channels, kind, None if offsets is None else offsets.data_ptr()
+        return rows, channels, kind, at, off
 
     def group_norm(self, x: torch.Tensor, weight, bias, groups: int, windows: int = 1, offsets=None,
                    eps: float = 1e-5, epilogue: int = EPI_NONE, flags: int = 0,
@@ -436,28 +452,30 @@ class Runtime:
         [rows, channels] in ``windows`` windows of equal length, or of the rows ``offsets[i]`` to
         ``offsets[i + 1] - 1`` (int32 on the device, ``windows + 1`` of them). Rows in no window are
         not written: ``out`` keeps what it held, and a new tensor has nothing there."""
-        rows, channels, kind, off = self._check_group_norm(x, weight, bias, windows, offsets)
+        rows, channels, kind, at, off = self._check_group_norm(x, weight, bias, windows, offsets)
         if out is None:
             out = torch.empty_like(x)
+            y = out.data_ptr()
         else:
-            self._check(out, 'out', x.dtype, x.shape)
-        need = self.lib.group_norm_workspace_size(rows, windows, channels, groups)
-        scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
-        self._call('pq8_group_norm', x.data_ptr(), kind, weight.data_ptr(), bias.data_ptr(), out.data_ptr(), rows,
-                   windows, off, channels, groups, float(eps), epilogue, flags, scratch.data_ptr(), need)
+            y = self._check(out, 'out', x.dtype, x.shape)
+        need = self.lib.group_norm_workspace_size(kind, rows, windows, channels, groups, False, not (at[0] | y) & 15)
+        scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._enqueue('pq8_group_norm', at[0], kind, at[1], at[2], y, rows, windows, off, channels, groups, eps,
+                      epilogue, flags, _ptr(scratch), need)
         return out
 
     def group_norm_quantize(self, x: torch.Tensor, weight, bias, groups: int, windows: int = 1, offsets=None,
                             eps: float = 1e-5, epilogue: int = EPI_NONE) -> QuantizedRows:
-        """``group_norm``, its rows quantised as ``quantize_rows`` does, for ``linear_i8``."""
-        rows, channels, kind, off = self._check_group_norm(x, weight, bias, windows, offsets)
+        """``group_norm``, its rows quantised as ``quantize_rows`` does, for ``linear_i8``. Rows in no window
+        have no values and no scale."""
+        rows, channels, kind, at, off = self._check_group_norm(x, weight, bias, windows, offsets)
         out = QuantizedRows(torch.empty(rows, channels, dtype=torch.int8, device=self.device),
                             torch.empty(rows, dtype=torch.float32, device=self.device))
-        need = self.lib.group_norm_workspace_size(rows, windows, channels, groups)
-        scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
-        self._call('pq8_group_norm_quantize', x.data_ptr(), kind, weight.data_ptr(), bias.data_ptr(),
-                   out.q.data_ptr(), out.scale.data_ptr(), rows, windows, off, channels, groups, float(eps), epilogue,
-                   scratch.data_ptr(), need)
+        need = self.lib.group_norm_workspace_size(kind, rows, windows, channels, groups, True,
+                                                  not (at[0] | at[1] | at[2]) & 15)
+        scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._enqueue('pq8_group_norm_quantize', at[0], kind, at[1], at[2], out.q_ptr, out.scale_ptr, rows, windows,
+                      off, channels, groups, eps, epilogue, _ptr(scratch), need)
         return out
 
     def device_status(self) -> int:

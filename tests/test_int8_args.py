@@ -89,16 +89,22 @@ def test_linear_i8_refusals(lib):
     assert need >= 4 * 64 + 16
     assert lib.linear_i8_workspace_size(0, 64) >= 0
     assert linear(lib, m=0, ws=None, size=0) == 0
-    assert linear(lib, ws=None) == pq8.ERR_WORKSPACE
-    assert linear(lib, size=need - 1) == pq8.ERR_WORKSPACE
+    need = lib.linear_i8_workspace_size(9, 64)
+    assert need == pq8.linear_i8_scratch(9, 64, 0) and pq8.linear_i8_scratch(8, 64, 0) == 0
+    assert pq8.linear_i8_scratch(8, 1040, 0) == lib.linear_i8_workspace_size(8, 1040)
+    assert pq8.linear_i8_scratch(1, 8192, 0) == 0 and pq8.linear_i8_scratch(1, 8208, 0) > 0
+    assert pq8.linear_i8_scratch(2, 64, 8) == lib.linear_i8_workspace_size(2, 64)
+    assert linear(lib, m=9, ws=None) == pq8.ERR_WORKSPACE
+    assert linear(lib, m=9, size=need - 1) == pq8.ERR_WORKSPACE
+    assert linear(lib, x=X + 4, ws=None) == pq8.ERR_WORKSPACE  # not the one-launch form
     assert linear(lib, ws=WS + 8) == pq8.ERR_MISALIGNED
     assert linear(lib, ld=60) == pq8.ERR_INVALID_ARGUMENT
     assert linear(lib, kind=-1) == pq8.ERR_INVALID_ARGUMENT
     assert linear(lib, nw=B) == pq8.ERR_INVALID_ARGUMENT  # weight without bias
     assert linear(lib, nb=B) == pq8.ERR_INVALID_ARGUMENT
     assert linear(lib, y=X + 128) == pq8.ERR_INVALID_ARGUMENT
-    assert linear(lib, x=WS) == pq8.ERR_INVALID_ARGUMENT  # tokens inside the workspace
-    assert linear(lib, y=WS + 64) == pq8.ERR_INVALID_ARGUMENT
+    assert linear(lib, m=9, x=WS) == pq8.ERR_INVALID_ARGUMENT  # tokens inside the workspace
+    assert linear(lib, m=9, y=WS + 64) == pq8.ERR_INVALID_ARGUMENT
     with pytest.raises(pq8.PQ8Error):
         lib.linear_i8_workspace_size(4, 65)
     assert code(lib, 'pq8_linear_i8_workspace_size', 4, 64, None) == pq8.ERR_INVALID_ARGUMENT
@@ -121,12 +127,14 @@ def test_group_norm_refusals(lib):
         assert norm(lib, **kw) == pq8.ERR_INVALID_ARGUMENT, kw
     for kw in ({'x': X + 2}, {'w': W + 2}, {'y': Y + 2}, {'y': Y + 1, 'kind': 2}, {'off': S + 2}, {'ws': WS + 8}):
         assert norm(lib, **kw) == pq8.ERR_MISALIGNED, kw
-    need = lib.group_norm_workspace_size(12, 3, 64, 4)
-    assert norm(lib, ws=None) == pq8.ERR_WORKSPACE
-    if need:
-        assert norm(lib, size=need - 1) == pq8.ERR_WORKSPACE
-    with pytest.raises(pq8.PQ8Error):
-        lib.group_norm_workspace_size(12, 3, 64, 5)
+    assert lib.group_norm_workspace_size(0, 12, 3, 64, 4) == 0  # one launch
+    need = lib.group_norm_workspace_size(0, 12, 3, 64, 4, quantize=True)
+    assert need >= 3 * 4 * 16 and lib.group_norm_workspace_size(0, 12, 3, 64, 4, aligned16=False) > 0
+    assert lib.group_norm_workspace_size(0, 0, 3, 64, 4) == lib.group_norm_workspace_size(0, 12, 0, 64, 4) == 0
+    for bad in ((0, 12, 3, 64, 5), (3, 12, 3, 64, 4), (0, -1, 3, 64, 4)):
+        with pytest.raises(pq8.PQ8Error):
+            lib.group_norm_workspace_size(*bad)
+    assert code(lib, 'pq8_group_norm_workspace_size', 0, 12, 3, 64, 4, 0, 1, None) == pq8.ERR_INVALID_ARGUMENT
     assert code(lib, 'pq8_group_norm_quantize', X, 0, W, B, Q, S, 12, 3, None, 60, 4, 1e-5, 0, WS, BIG,
                 None) == pq8.ERR_UNSUPPORTED_SHAPE
     assert code(lib, 'pq8_group_norm_quantize', X, 0, W, B, Q, None, 12, 3, None, 64, 4, 1e-5, 0, WS, BIG,
