@@ -529,19 +529,20 @@ PQ8_API int pq8_linear_i8(const int8_t* w, const float* w_scale, const void* x, 
  * channels / groups channels of one group, y = act((x - mean) / sqrt(var +
  * eps) * w + b) with act PQ8_EPI_NONE, PQ8_EPI_RELU or PQ8_EPI_SILU. w, b:
  * float[channels]. offsets: device int[windows + 1], window i has rows
- * offsets[i] to offsets[i + 1] - 1 (windows of no rows are fine; they should
- * not overlap: a row in two windows gets the values of either; an offset
- * outside 0..rows is held to that range, and a window that ends before it
- * starts is empty), rows of y in no window are not written; or NULL: windows of rows / windows rows each.
- * Sums are FP64, in a fixed order. channels at most 16384, groups at most
+ * offsets[i] to offsets[i + 1] - 1 (windows of no rows are fine; an offset
+ * outside 0..rows is held to that range; offsets must not fall: the rows
+ * concerned would get no defined values, though nothing outside y is touched),
+ * rows of y in no window are not written; or NULL: windows of rows / windows rows each.
+ * Sums are added in a fixed order, per column over at most 32 rows in FP32 (FP64
+ * for the quantised form), FP64 above. channels at most 16384, groups at most
  * 4096, rows at most 2^30. y must not overlap x. PQ8_FLAG_OUT_TF32 (type F32)
  * rounds y for a following pq8_gemm. The workspace (16-byte aligned, no
  * initialisation) is per call in flight; where its size is 0 it may be NULL.
- * quantize: 1 for pq8_group_norm_quantize; aligned16: whether x and y (x, w
+ * ragged: 1 with offsets; quantize: 1 for pq8_group_norm_quantize; aligned16: whether x and y (x, w
  * and b with quantize) start on 16-byte boundaries. No counterpart in the reference,
  * whose conv module has BatchNorm (reference.py:60-63). */
-PQ8_API int pq8_group_norm_workspace_size(int type, int rows, int windows, int channels, int groups, int quantize,
-                                          int aligned16, size_t* bytes);
+PQ8_API int pq8_group_norm_workspace_size(int type, int rows, int windows, int channels, int groups, int ragged,
+                                          int quantize, int aligned16, size_t* bytes);
 PQ8_API int pq8_group_norm(const void* x, int type, const float* w, const float* b, void* y, int rows, int windows,
                            const int* offsets, int channels, int groups, double eps, int activation, int flags,
                            void* workspace, size_t workspace_bytes, void* stream);

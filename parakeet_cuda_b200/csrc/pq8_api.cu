@@ -2250,17 +2250,30 @@ int i8_tensor_map(EncodeTiledFn enc, CUtensorMap* map, const int8_t* base, int r
   return r == CUDA_SUCCESS ? PQ8_OK : PQ8_ERR_DRIVER;
 }
 
-template <typename T, int BN, bool PAIR, int STAGES>
+template <typename T, int BN, bool PAIR>
 int launch_i8_gemm(DeviceState* ds, const I8Params& p, int splits, cudaStream_t st) {
-  using C = I8Cfg<BN, PAIR, STAGES>;
+  using C = I8Cfg<BN, PAIR>;
   EncodeTiledFn enc;
   int rc = encode_fn(&enc);
   if (rc) return rc;
   CUtensorMap wmap, xmap;
-  if ((rc = i8_tensor_map(enc, &wmap, p.w, p.n, p.k, p.epi == PQ8_EPI_GLU ? 16 : 128))) return rc;
-  if ((rc = i8_tensor_map(enc, &xmap, p.x, p.m, p.k, C::kTokens))) return rc;
   I8GemmParams g{};
   g.p = p;
+  // GLU weights as [blocks of 16 channels][value, gate][16][k], if the halves are whole blocks
+  g.glu_blocks = p.epi == PQ8_EPI_GLU && p.out_cols % 16 == 0;
+  if (g.glu_blocks) {
+    const cuuint64_t k64 = static_cast<cuuint64_t>(p.k);
+    const cuuint64_t dims[4] = {k64, 16, 2, static_cast<cuuint64_t>(p.out_cols / 16)};
+    const cuuint64_t strides[3] = {k64, k64 * p.out_cols, k64 * 16};
+    const cuuint32_t box[4] = {128, 16, 2, 4}, estr[4] = {1, 1, 1, 1};
+    if (enc(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(p.w), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return PQ8_ERR_DRIVER;
+  } else if ((rc = i8_tensor_map(enc, &wmap, p.w, p.n, p.k, p.epi == PQ8_EPI_GLU ? 16 : 128))) {
+    return rc;
+  }
+  if ((rc = i8_tensor_map(enc, &xmap, p.x, p.m, p.k, C::kTokens))) return rc;
   g.n_tiles = p.epi == PQ8_EPI_GLU ? (p.out_cols + 63) / 64 : (p.n + 127) / 128;
   g.m_tiles = (p.m + BN - 1) / BN;
   g.k_blocks = (p.k + 127) / 128;
@@ -2271,7 +2284,7 @@ int launch_i8_gemm(DeviceState* ds, const I8Params& p, int splits, cudaStream_t 
   // a split CTA runs one tile (its sums take the place of the loads)
   const long long slots = ds->sms / per;
   if (splits > 1 && tiles > slots) return PQ8_ERR_INVALID_ARGUMENT;
-  auto kernel = i8_gemm_kernel<T, BN, PAIR, STAGES>;
+  auto kernel = i8_gemm_kernel<T, BN, PAIR>;
   static bool attr_set[kMaxDevices];
   const cudaError_t ea = allow_smem(kernel, C::kSmemBytes, attr_set);
   if (ea != cudaSuccess) return to_code(ea);
@@ -2294,26 +2307,108 @@ int launch_i8_gemm(DeviceState* ds, const I8Params& p, int splits, cudaStream_t 
   return to_code(cudaGetLastError());
 }
 
-// K splits for a tile count: 2, 4 or 8 CTAs a tile while they fit the SMs and
-// each keeps at least two 128-value blocks.
-int i8_splits(int tiles, int k_blocks, int sms) {
-  int s = 1;
-  while (s < 8 && tiles * s * 2 <= sms && k_blocks >= 4 * s && (2 * s - 1) * ((k_blocks + 2 * s - 1) / (2 * s)) < k_blocks)
-    s *= 2;
-  return s;
+// Tile shapes (tokens per tile; a CTA or a pair of them) with a model of a launch's
+// time in us: fixed + waves x (K blocks of 128 x per_block + per_tile), and, with K
+// split over a cluster, split. Fitted to B200 times of 16 to 12,000 tokens, K
+// 640 to 16,384: e.g. 375 x 1024 x 1024 (tokens x K x channels) takes 5.1 us in
+// tiles of 32, 6.0 of 128, 7.3 of 256; 375 x 4096 x 1024 11.5 in tiles of 32 and
+// 9.9 of 128 with K in 4 splits; 3000 x 4096 x 1024 24 of 128, 17.4 of 192, 19.3
+// of 256; 12,000 x 1024 x 1024 49 of 32, 23 of 128, 19.6 of 192, 18.2 of 256.
+struct I8Shape {
+  int tokens, ctas;
+  double fixed, per_block, per_tile, split;
+};
+constexpr I8Shape kI8Shapes[] = {{16, 1, 3.0, 0.255, 0.1, 1.1},  {32, 1, 3.0, 0.255, 0.15, 1.4},
+                                 {64, 1, 3.2, 0.255, 0.45, 1.9}, {128, 1, 3.9, 0.26, 1.1, 2.5},
+                                 {192, 2, 4.4, 0.27, 1.6, 0.0},  {256, 2, 3.4, 0.31, 2.2, 0.0}};
+
+struct I8Choice {
+  int shape, splits;
+};
+
+// How many clusters of `splits` CTAs of a tile shape the GPU holds at once (a
+// CTA fills an SM, and a cluster lies within one group of SMs). Asked once per
+// device; the query enqueues nothing, and relaxed capture mode lets it run
+// while the caller's stream is captured.
+template <int BN>
+int i8_cluster_fit(DeviceState* ds, int splits) {
+  using C = I8Cfg<BN, false>;
+  const long long key = (1LL << 62) | (static_cast<long long>(BN) << 8) | splits;  // apart from the GEMV's keys
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    auto it = ds->gemv_cluster_fit.find(key);
+    if (it != ds->gemv_cluster_fit.end()) return it->second;
+  }
+  auto kernel = i8_gemm_kernel<float, BN, false>;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  int n = 0;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits);
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  }
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return 0;  // no answer: no split
+  }
+  std::lock_guard<std::mutex> lock(g_mutex);
+  ds->gemv_cluster_fit[key] = n;
+  return n;
+}
+
+I8Choice choose_i8(DeviceState* ds, int m, int n_tiles, int k_blocks) {
+  const int sms = ds->sms;
+  auto fit = [&](int shape, int splits) {
+    return shape == 0   ? i8_cluster_fit<16>(ds, splits)
+           : shape == 1 ? i8_cluster_fit<32>(ds, splits)
+           : shape == 2 ? i8_cluster_fit<64>(ds, splits)
+                        : i8_cluster_fit<128>(ds, splits);
+  };
+  I8Choice best{0, 1};
+  double least = -1.0;
+  for (int c = 0; c < static_cast<int>(sizeof(kI8Shapes) / sizeof(kI8Shapes[0])); ++c) {
+    const I8Shape& s = kI8Shapes[c];
+    const long long tiles =
+        static_cast<long long>((n_tiles + s.ctas - 1) / s.ctas) * ((m + s.tokens - 1) / s.tokens);
+    for (int splits = 1; splits <= (s.ctas == 1 ? 8 : 1); splits *= 2) {
+      const int per = (k_blocks + splits - 1) / splits;
+      // a split launch is one wave, and every split has K blocks
+      if (splits > 1 && (tiles * splits > sms || (splits - 1) * per >= k_blocks || tiles > fit(c, splits))) break;
+      const long long slots = sms / s.ctas, waves = splits > 1 ? 1 : (tiles + slots - 1) / slots;
+      const double cost = s.fixed + waves * (per * s.per_block + s.per_tile) + (splits > 1 ? s.split : 0.0);
+      if (least < 0.0 || cost < least) {
+        least = cost;
+        best = {c, splits};
+      }
+    }
+  }
+  return best;
 }
 
 template <typename T>
 int launch_i8_tiles(DeviceState* ds, const I8Params& p, cudaStream_t st) {
   const int n_tiles = p.epi == PQ8_EPI_GLU ? (p.out_cols + 63) / 64 : (p.n + 127) / 128;
-  const int k_blocks = (p.k + 127) / 128;
-  const long long tiles128 = static_cast<long long>(n_tiles) * ((p.m + 127) / 128);
-  if (tiles128 > ds->sms) return launch_i8_gemm<T, 256, true, 6>(ds, p, 1, st);
-  const int splits = i8_splits(static_cast<int>(p.m <= 64 ? n_tiles : tiles128), k_blocks, ds->sms);
-  if (p.m <= 16 && n_tiles <= ds->sms / splits) return launch_i8_gemm<T, 16, false, 8>(ds, p, splits, st);
-  if (p.m <= 32) return launch_i8_gemm<T, 32, false, 8>(ds, p, splits, st);
-  if (p.m <= 64) return launch_i8_gemm<T, 64, false, 8>(ds, p, splits, st);
-  return launch_i8_gemm<T, 128, false, 6>(ds, p, splits, st);
+  const I8Choice c = choose_i8(ds, p.m, n_tiles, (p.k + 127) / 128);
+  switch (c.shape) {
+    case 0: return launch_i8_gemm<T, 16, false>(ds, p, c.splits, st);
+    case 1: return launch_i8_gemm<T, 32, false>(ds, p, c.splits, st);
+    case 2: return launch_i8_gemm<T, 64, false>(ds, p, c.splits, st);
+    case 3: return launch_i8_gemm<T, 128, false>(ds, p, c.splits, st);
+    case 4: return launch_i8_gemm<T, 192, true>(ds, p, 1, st);
+    default: return launch_i8_gemm<T, 256, true>(ds, p, 1, st);
+  }
 }
 
 int launch_i8(DeviceState* ds, const I8Params& p, int y_type, cudaStream_t st) {
@@ -2447,7 +2542,7 @@ struct GroupNormPlan {
   int parts;          // one launch: CTAs of a window's cluster; 0: two launches
   int hold;           // one launch: rows a CTA holds
   size_t smem;        // one launch
-  int chunks, apply;  // two launches: row chunks of the sums, and of the second launch
+  int block, row_block;  // two launches: rows a CTA takes, for the sums and in the second launch
   size_t total;       // workspace
 };
 
@@ -2455,7 +2550,8 @@ constexpr size_t kNormMaxSmem = size_t(200) << 10;
 
 // `vec`: 16-byte loads fit the addresses. The same for every device, so that the
 // workspace can be sized without one.
-GroupNormPlan plan_group_norm(int size, bool vec, int rows, int windows, int channels, int groups, bool quantize) {
+GroupNormPlan plan_group_norm(int size, bool vec, int rows, int windows, bool ragged, int channels, int groups,
+                              bool quantize) {
   constexpr int sms = 148;
   GroupNormPlan g{};
   const int cg = channels / groups, E = 16 / size;
@@ -2482,25 +2578,29 @@ GroupNormPlan plan_group_norm(int size, bool vec, int rows, int windows, int cha
   const size_t row_bytes = static_cast<size_t>(g.slab) * cg * size;
   if (!quantize && g.units != kScalar && windows <= 65535) {
     // One launch: the smallest cluster that holds an average window at four
-    // CTAs an SM, and that gives every SM a CTA; at most 8 CTAs.
+    // CTAs an SM, and that gives every SM a CTA; at most 8 CTAs. Windows of
+    // unequal lengths take it only where its CTAs are many enough to even out.
     int parts = 1;
     while (parts < 8 && ((t + parts - 1) / parts * row_bytes > (48 << 10) ||
                          (units * parts < sms && t / (2 * parts) >= 16)))
       parts *= 2;
     const int per = (t + parts - 1) / parts;
     const size_t tables = static_cast<size_t>(g.slab) * (sizeof(GroupSum) + sizeof(GroupStat));
-    if (per * row_bytes + tables <= kNormMaxSmem) {
+    if (per * row_bytes + tables <= kNormMaxSmem && (!ragged || windows == 1 || units * parts >= 8LL * sms)) {
       g.parts = parts;
       g.hold = per;
       g.smem = per * row_bytes + tables;
       return g;
     }
   }
-  // Two launches: row chunks that fill the SMs a few times, eight rows at least.
-  const long long fill = std::max<long long>(1, 8LL * sms / units);
-  g.chunks = static_cast<int>(std::min<long long>({64, (t + 7) / 8, fill}));
-  g.apply = static_cast<int>(std::min<long long>((t + 7) / 8, quantize ? std::max<long long>(1, 6LL * sms / std::max(windows, 1)) : fill));
-  g.total = round256(sizeof(GroupSum) * static_cast<size_t>(windows) * g.chunks * groups);
+  // Two launches: blocks of rows that fill the SMs a few times. (Rows to
+  // quantise stay whole: their second launch has no slabs.)
+  auto block = [&](long long slabs, int ctas, int least_rows) {
+    return static_cast<int>(std::max<long long>(least_rows, (std::max(rows, 1) * slabs + ctas - 1) / ctas));
+  };
+  g.block = block(g.slabs, 4 * sms, 16);
+  g.row_block = quantize ? block(1, 4 * sms, 8) : g.block;
+  g.total = round256(sizeof(GroupSum) * (static_cast<size_t>((rows + g.block - 1) / g.block) + windows) * groups);
   return g;
 }
 
@@ -2551,9 +2651,10 @@ GroupNormParams group_norm_params(const GroupNormPlan& g, const void* x, const f
   p.groups = groups;
   p.epi = act;
   p.eps = eps;
-  p.chunks = g.chunks;
   p.slab = g.slab;
   p.hold = g.hold;
+  p.block = g.block;
+  p.row_block = g.row_block;
   return p;
 }
 
@@ -2590,25 +2691,25 @@ cudaError_t launch_group_norm_one(const GroupNormPlan& g, const GroupNormParams&
   return cudaLaunchKernelEx(&cfg, kernel, p, y);
 }
 
-template <typename T>
+template <typename T, bool EXACT>
 cudaError_t launch_group_stats(const GroupNormPlan& g, const GroupNormParams& p, GroupSum* partial, cudaStream_t st) {
-  const dim3 grid(g.chunks, std::min(p.windows, 65535), g.slabs);
+  const dim3 grid((p.rows + g.block - 1) / g.block, g.slabs);
   return with_units(g.units, [&](auto u) {
-    return launch_pdl(group_stats_kernel<T, decltype(u)::value>, grid, dim3(kNormThreads), 0, st, p, partial);
+    return launch_pdl(group_stats_kernel<T, decltype(u)::value, EXACT>, grid, dim3(kNormThreads), 0, st, p, partial);
   });
 }
 
 }  // namespace
 }  // namespace pq8
 
-extern "C" int pq8_group_norm_workspace_size(int type, int rows, int windows, int channels, int groups, int quantize,
-                                             int aligned16, size_t* bytes) {
+extern "C" int pq8_group_norm_workspace_size(int type, int rows, int windows, int channels, int groups, int ragged,
+                                             int quantize, int aligned16, size_t* bytes) {
   if (bytes == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
   const int rc = check_group_norm_shape(type, rows, windows, channels, groups);
   if (rc) return rc;
   *bytes = 0;
   if (rows > 0 && windows > 0)
-    *bytes = plan_group_norm(type_size(type), aligned16 != 0, rows, windows, channels, groups, quantize != 0).total;
+    *bytes = plan_group_norm(type_size(type), aligned16 != 0, rows, windows, ragged != 0, channels, groups, quantize != 0).total;
   return PQ8_OK;
 }
 
@@ -2625,8 +2726,8 @@ extern "C" int pq8_group_norm(const void* x, int type, const float* w, const flo
   if (!aligned(y, type_size(type))) return PQ8_ERR_MISALIGNED;
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
-  const GroupNormPlan g = plan_group_norm(type_size(type), aligned(x, 16) && aligned(y, 16), rows, windows, channels,
-                                          groups, false);
+  const GroupNormPlan g = plan_group_norm(type_size(type), aligned(x, 16) && aligned(y, 16), rows, windows,
+                                          offsets != nullptr, channels, groups, false);
   if ((rc = check_norm_workspace(g, workspace, workspace_bytes, x, bytes, y, bytes))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(type, [&](auto t) {
@@ -2637,9 +2738,9 @@ extern "C" int pq8_group_norm(const void* x, int type, const float* w, const flo
       return g.units == kWhole ? launch_group_norm_one<T, kWhole>(g, p, static_cast<T*>(y), st)
                                : launch_group_norm_one<T, kStraddle>(g, p, static_cast<T*>(y), st);
     GroupSum* partial = static_cast<GroupSum*>(workspace);
-    const cudaError_t err = launch_group_stats<T>(g, p, partial, st);
+    const cudaError_t err = launch_group_stats<T, false>(g, p, partial, st);
     if (err != cudaSuccess) return err;
-    const dim3 grid(g.apply, std::min(windows, 65535), g.slabs);
+    const dim3 grid((rows + g.row_block - 1) / g.row_block, g.slabs);
     return with_units(g.units, [&](auto u) {
       return launch_pdl(group_apply_kernel<T, decltype(u)::value>, grid, dim3(kNormThreads),
                         sizeof(GroupStat) * g.slab, st, p, static_cast<const GroupSum*>(partial), static_cast<T*>(y));
@@ -2665,16 +2766,17 @@ extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, 
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
   const bool vec = aligned(x, 16) && aligned(w, 16) && aligned(b, 16);
-  const GroupNormPlan g = plan_group_norm(type_size(type), vec, rows, windows, channels, groups, true);
+  const GroupNormPlan g =
+      plan_group_norm(type_size(type), vec, rows, windows, offsets != nullptr, channels, groups, true);
   if ((rc = check_norm_workspace(g, workspace, workspace_bytes, x, x_bytes, q, q_bytes))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
     const GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
     GroupSum* partial = static_cast<GroupSum*>(workspace);
-    cudaError_t err = launch_group_stats<T>(g, p, partial, st);
+    cudaError_t err = launch_group_stats<T, true>(g, p, partial, st);
     if (err != cudaSuccess) return err;
-    const dim3 grid(g.apply, std::min(windows, 65535));
+    const dim3 grid((rows + g.row_block - 1) / g.row_block);
     const size_t smem = (sizeof(GroupStat) + sizeof(float4)) * groups;
     constexpr int C = 32 / kChunk<T>;
     auto kernel = !vec               ? group_quantize_kernel<T, 0, 8, false>

@@ -3,9 +3,13 @@
 // rows; mean and variance over the rows of one window and the channels of one
 // group,
 //   y = act((x - mean) / sqrt(var + eps) * w + b).
-// Sums are fp64, taken of x minus the group's first value of the window, so
-// that neither a large common offset nor a long window costs digits; they are
-// added in a fixed order.
+// Sums are taken of x minus a nearby value, so that neither a large common
+// offset nor a long window costs digits, and added in a fixed order: per
+// column over at most 32 rows of a thread in fp32 (minus the first of them;
+// two columns per instruction, no conversions), everything above in fp64
+// (minus the group's first value of the window). Where the result is
+// quantised every value goes to fp64 at once: integers next to a border need
+// the statistics to more digits.
 //
 // Two forms. Where a window's rows of a few groups fit the shared memory of a
 // cluster, one launch reads x once: every CTA holds its rows there, the
@@ -25,7 +29,8 @@ struct GroupNormParams {
   const int* offsets;  // [windows + 1], or NULL: windows of rows / windows rows
   int rows, windows, channels, groups, epi, round_out;
   double eps;
-  int chunks;      // two launches: row chunks per window of the sums
+  int block;       // two launches: rows a CTA of the sums takes, whatever windows they belong to
+  int row_block;   // two launches: the same in the second launch
   int slab;        // whole groups per CTA; their columns are whole units
   int hold;        // one launch: rows a CTA holds in shared memory
 };
@@ -86,21 +91,73 @@ __device__ __forceinline__ void unit_group(int u, int cg, int* g, int* split) {
   *split = UNITS == kStraddle ? min((*g + 1) * cg - u * E, E) : E;
 }
 
-template <int UNITS, int E>
-__device__ __forceinline__ void add_unit(GroupSum2& acc, const float (&v)[E], int split, double fa, double fb) {
+// A thread's sums of one unit's columns over its rows, into acc by flush().
+// EXACT: every value in fp64 at once.
+template <int UNITS, int E, bool EXACT>
+struct UnitSum {
+  static constexpr int kRun = 32;  // rows in fp32
+  static constexpr int H = E > 1 ? E / 2 : 1;
+  int split, run = 0;
+  double fa, fb;  // first values of the unit's first group and of the next
+  f32x2 minus[H], s[H], q[H];  // minus the run's first row; sums of the differences and of their squares
+  __device__ __forceinline__ UnitSum(int split_, double fa_, double fb_) : split(split_), fa(fa_), fb(fb_) {}
+  __device__ __forceinline__ void add(GroupSum2& acc, const float (&v)[E]) {
+    if constexpr (EXACT) {
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    if (UNITS != kStraddle || i < split) {
-      const double d = static_cast<double>(v[i]) - fa;
-      acc.a.s += d;
-      acc.a.q += d * d;
+      for (int i = 0; i < E; ++i) {
+        const bool next = UNITS == kStraddle && i >= split;
+        const double d = static_cast<double>(v[i]) - (next ? fb : fa);
+        if (next) {
+          acc.b.s += d;
+          acc.b.q += d * d;
+        } else {
+          acc.a.s += d;
+          acc.a.q += d * d;
+        }
+      }
     } else {
-      const double d = static_cast<double>(v[i]) - fb;
-      acc.b.s += d;
-      acc.b.q += d * d;
+      if (run == 0) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          minus[i] = pack2(-v[2 * i], E > 1 ? -v[2 * i + (E > 1)] : 0.0f);
+          s[i] = q[i] = 0;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const f32x2 d = add2(pack2(v[2 * i], E > 1 ? v[2 * i + (E > 1)] : 0.0f), minus[i]);
+        s[i] = add2(s[i], d);
+        q[i] = fma2(d, d, q[i]);
+      }
+      if (++run == kRun) flush(acc);
     }
   }
-}
+  __device__ __forceinline__ void flush(GroupSum2& acc) {
+    if constexpr (!EXACT) {
+      if (run == 0) return;
+      const double n = run;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        float m[2], ss[2], qq[2];
+        unpack2(minus[i / 2], &m[0], &m[1]);
+        unpack2(s[i / 2], &ss[0], &ss[1]);
+        unpack2(q[i / 2], &qq[0], &qq[1]);
+        const bool next = UNITS == kStraddle && i >= split;
+        // off: the run's reference value minus the group's
+        const double off = -static_cast<double>(m[i % 2]) - (next ? fb : fa), sd = static_cast<double>(ss[i % 2]);
+        const double ds = sd + n * off, dq = static_cast<double>(qq[i % 2]) + off * (2.0 * sd + n * off);
+        if (next) {
+          acc.b.s += ds;
+          acc.b.q += dq;
+        } else {
+          acc.a.s += ds;
+          acc.a.q += dq;
+        }
+      }
+      run = 0;
+    }
+  }
+};
 
 // The threads' sums of the slab's ng groups to out[g], a warp per group, in a
 // fixed order. All threads of the CTA; red: kNormThreads entries.
@@ -141,39 +198,44 @@ __device__ __forceinline__ double first_value(const GroupNormParams& p, int lo, 
       to_f32(static_cast<const T*>(p.x)[static_cast<size_t>(lo) * p.channels + static_cast<size_t>(g0 + g) * cg]));
 }
 
-// Normalisation of one unit: mean and 1 / deviation in fp32 (the mean in two
-// parts, so that x - mean is rounded relative to its own size), weight, bias.
+// Normalisation of one unit's columns: y = act((x - hi) a + c) with hi the mean
+// rounded to fp32 (x - hi is rounded relative to its own size, whatever the
+// mean), a = w / deviation, and c = b minus what is left of the mean.
 template <int UNITS, int E>
 struct UnitNorm {
-  float hi_a, lo_a, rs_a, hi_b, lo_b, rs_b;  // of the unit's first group and of the next
-  float g[E], h[E];
+  float hi_a, hi_b;  // of the unit's first group and of the next
+  float a[E], c[E];
   int split;
   __device__ __forceinline__ UnitNorm(const GroupNormParams& p, const GroupStat* stat, int u, int cg, int ng, int col) {
     int first;
     unit_group<UNITS, E>(u, cg, &first, &split);
-    set(stat[first], &hi_a, &lo_a, &rs_a);
-    if constexpr (UNITS == kStraddle) set(stat[min(first + 1, ng - 1)], &hi_b, &lo_b, &rs_b);
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      g[i] = p.w[col + i];
-      h[i] = p.b[col + i];
-    }
-  }
-  __device__ __forceinline__ static void set(const GroupStat& st, float* hi, float* lo, float* rs) {
-    *hi = static_cast<float>(st.mean);
-    *lo = static_cast<float>(st.mean - static_cast<double>(*hi));
-    *rs = static_cast<float>(st.rstd);
-  }
-  __device__ __forceinline__ void apply(float (&v)[E], int epi, int round_out) const {
+    const GroupStat sa = stat[first], sb = UNITS == kStraddle ? stat[min(first + 1, ng - 1)] : sa;
+    hi_a = static_cast<float>(sa.mean);
+    hi_b = static_cast<float>(sb.mean);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const bool next = UNITS == kStraddle && i >= split;
-      v[i] = fmaf(((v[i] - (next ? hi_b : hi_a)) - (next ? lo_b : lo_a)) * (next ? rs_b : rs_a), g[i], h[i]);
+      const double rest = next ? sb.mean - static_cast<double>(hi_b) : sa.mean - static_cast<double>(hi_a);
+      const double scale = (next ? sb.rstd : sa.rstd) * static_cast<double>(p.w[col + i]);
+      a[i] = static_cast<float>(scale);
+      c[i] = static_cast<float>(static_cast<double>(p.b[col + i]) - rest * scale);
     }
-    if (epi == PQ8_EPI_SILU) {
+  }
+  __device__ __forceinline__ void apply(float (&v)[E], int epi, int round_out) const {
+    if constexpr (E == 1) {
+      v[0] = fmaf(v[0] - hi_a, a[0], c[0]);
+      if (epi == PQ8_EPI_SILU) v[0] = act_f32(v[0], PQ8_EPI_SILU);
+    } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = act_f32(v[i], PQ8_EPI_SILU);
-    } else if (epi == PQ8_EPI_RELU) {
+      for (int i = 0; i < E; i += 2) {
+        const f32x2 hi = pack2(-(UNITS == kStraddle && i >= split ? hi_b : hi_a),
+                               -(UNITS == kStraddle && i + 1 >= split ? hi_b : hi_a));
+        f32x2 z = fma2(add2(pack2(v[i], v[i + 1]), hi), pack2(a[i], a[i + 1]), pack2(c[i], c[i + 1]));
+        if (epi == PQ8_EPI_SILU) z = mul2(z, sigmoid2(z));
+        unpack2(z, &v[i], &v[i + 1]);
+      }
+    }
+    if (epi == PQ8_EPI_RELU) {
 #pragma unroll
       for (int i = 0; i < E; ++i) v[i] = act_f32(v[i], PQ8_EPI_RELU);
     }
@@ -204,7 +266,6 @@ __device__ __forceinline__ void store_unit(T* p, const float (&v)[kUnit<T, UNITS
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
   double v;
   asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
@@ -230,33 +291,50 @@ __global__ void __launch_bounds__(kNormThreads)
   const int held_end = min(r1, r0 + p.hold);
   const T* const x = static_cast<const T*>(p.x) + static_cast<size_t>(g0) * cg;
   const bool active = sh.y < sh.ty;
-  // a thread reads back only what it has put there itself
-  if (active) {
-    for (int u = sh.x; u < sh.units; u += sh.tx)
-      for (int r = r0 + sh.y; r < held_end; r += sh.ty)
+  // A thread reads back only what it has put there itself, so no barrier. Its
+  // rows arrive in four groups; the sums of one are taken while the next are
+  // under way. (Several units per thread: a slab of one wide group.)
+  const int mine = active && held_end > r0 + sh.y ? (held_end - r0 - sh.y + sh.ty - 1) / sh.ty : 0;
+  const int quarter = (mine + 3) / 4;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    for (int i = k * quarter; i < min(mine, (k + 1) * quarter); ++i) {
+      const int r = r0 + sh.y + i * sh.ty;
+      for (int u = sh.x; u < sh.units; u += sh.tx)
         cp_async16(held + static_cast<size_t>(r - r0) * sh.units + u, x + static_cast<size_t>(r) * p.channels + u * E);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
   GroupSum2 acc{{0.0, 0.0}, {0.0, 0.0}};
-  if (active) {
-    for (int u = sh.x; u < sh.units; u += sh.tx) {
-      int g, split;
-      unit_group<UNITS, E>(u, cg, &g, &split);
-      const double fa = first_value<T>(p, lo, hi, g0, g, cg);
-      const double fb = UNITS == kStraddle && split < E ? first_value<T>(p, lo, hi, g0, g + 1, cg) : 0.0;
-      float v[E];
-      for (int r = held_end + sh.y; r < r1; r += sh.ty) {
-        load_unit<T, UNITS>(x + static_cast<size_t>(r) * p.channels + u * E, v);
-        add_unit<UNITS, E>(acc, v, split, fa, fb);
-      }
-      cp_async_wait_all();
-#pragma unroll 4
-      for (int r = r0 + sh.y; r < held_end; r += sh.ty) {
-        load_unit<T, UNITS>(reinterpret_cast<const T*>(held + static_cast<size_t>(r - r0) * sh.units + u), v);
-        add_unit<UNITS, E>(acc, v, split, fa, fb);
+  int g, split;
+  unit_group<UNITS, E>(min(sh.x, sh.units - 1), cg, &g, &split);  // the same for all of a thread's units
+  UnitSum<UNITS, E, false> sum(split, first_value<T>(p, lo, hi, g0, g, cg),
+                               UNITS == kStraddle && split < E ? first_value<T>(p, lo, hi, g0, g + 1, cg) : 0.0);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (k == 0) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (k == 1) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (k == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll 2
+    for (int i = k * quarter; i < min(mine, (k + 1) * quarter); ++i) {
+      const int r = sh.y + i * sh.ty;
+      for (int u = sh.x; u < sh.units; u += sh.tx) {
+        float v[E];
+        load_unit<T, UNITS>(reinterpret_cast<const T*>(held + static_cast<size_t>(r) * sh.units + u), v);
+        sum.add(acc, v);
       }
     }
   }
-  cp_async_wait_all();
+  if (active) {
+    for (int r = held_end + sh.y; r < r1; r += sh.ty)
+      for (int u = sh.x; u < sh.units; u += sh.tx) {
+        float v[E];
+        load_unit<T, UNITS>(x + static_cast<size_t>(r) * p.channels + u * E, v);
+        sum.add(acc, v);
+      }
+  }
+  sum.flush(acc);
   reduce_groups<UNITS, E>(sh, acc, cg, ng, red, sums);
   // every CTA adds the parts' sums in the same order
   if (parts > 1) cluster_sync();
@@ -302,29 +380,58 @@ __global__ void __launch_bounds__(kNormThreads)
 }
 
 // ---------------------------------------------------------------------------
-// Two launches. Partial sums of one row chunk of one window for the groups of
-// one slab: partial[window][chunk][group].
-template <typename T, int UNITS>
+// Two launches. CTAs take blocks of rows of the whole buffer, so that windows
+// of any lengths keep them equally busy; a block's rows are worked through
+// window by window. The sums of block b and window w go to partial[b + w]
+// (blocks and windows both follow the rows, so no two pairs meet there).
+
+// f(window, its rows [lo, hi), those within [b0, b1)) for the windows with
+// rows in [b0, b1). Every thread of the CTA takes part.
+template <typename F>
+__device__ __forceinline__ void block_windows(const GroupNormParams& p, int b0, int b1, F&& f) {
+  int w = 0;
+  if (p.offsets == nullptr) {
+    w = b0 / (p.rows / p.windows);
+  } else {
+    // the windows that end at or before b0 come first
+    for (int i0 = 0; i0 < p.windows; i0 += blockDim.x) {
+      const int i = i0 + static_cast<int>(threadIdx.x);
+      const int n = __syncthreads_count(i < p.windows && p.offsets[i + 1] <= b0);
+      w += n;
+      if (n < static_cast<int>(blockDim.x)) break;
+    }
+  }
+  for (; w < p.windows; ++w) {
+    int lo, hi;
+    window_rows(p, w, &lo, &hi);
+    if (lo >= b1) break;
+    const int r0 = max(lo, b0), r1 = min(hi, b1);
+    if (r0 < r1) f(w, lo, hi, r0, r1);
+  }
+}
+
+// Sums of one block of rows for the groups of one slab.
+template <typename T, int UNITS, bool EXACT>
 __global__ void __launch_bounds__(kNormThreads)
     group_stats_kernel(const GroupNormParams p, GroupSum* __restrict__ partial) {
   constexpr int E = kUnit<T, UNITS>;
   __shared__ GroupSum2 red[kNormThreads];
   griddep_wait();
   griddep_launch();
-  const int cg = p.channels / p.groups, g0 = static_cast<int>(blockIdx.z) * p.slab, ng = min(p.slab, p.groups - g0);
+  const int cg = p.channels / p.groups, g0 = static_cast<int>(blockIdx.y) * p.slab, ng = min(p.slab, p.groups - g0);
   const SlabShape<E> sh(ng * cg);
   const T* const x = static_cast<const T*>(p.x) + static_cast<size_t>(g0) * cg;
-  for (int w = blockIdx.y; w < p.windows; w += gridDim.y) {
-    int lo, hi, r0, r1;
-    window_rows(p, w, &lo, &hi);
-    part_rows(lo, hi, blockIdx.x, p.chunks, &r0, &r1);
+  const int b0 = static_cast<int>(blockIdx.x) * p.block;
+  const int b1 = static_cast<int>(min(static_cast<long long>(b0) + p.block, static_cast<long long>(p.rows)));
+  block_windows(p, b0, b1, [&](int w, int lo, int hi, int r0, int r1) {
     GroupSum2 acc{{0.0, 0.0}, {0.0, 0.0}};
     if (sh.y < sh.ty) {
       for (int u = sh.x; u < sh.units; u += sh.tx) {
         int g, split;
         unit_group<UNITS, E>(u, cg, &g, &split);
-        const double fa = first_value<T>(p, lo, hi, g0, g, cg);
-        const double fb = UNITS == kStraddle && split < E ? first_value<T>(p, lo, hi, g0, g + 1, cg) : 0.0;
+        UnitSum<UNITS, E, EXACT> sum(
+            split, first_value<T>(p, lo, hi, g0, g, cg),
+            UNITS == kStraddle && split < E ? first_value<T>(p, lo, hi, g0, g + 1, cg) : 0.0);
         const T* const xu = x + u * E;
         constexpr int kAhead = 4;  // rows whose loads are issued together
         int r = r0 + sh.y;
@@ -334,42 +441,58 @@ __global__ void __launch_bounds__(kNormThreads)
           for (int k = 0; k < kAhead; ++k)
             load_unit<T, UNITS>(xu + static_cast<size_t>(r + k * sh.ty) * p.channels, v[k]);
 #pragma unroll
-          for (int k = 0; k < kAhead; ++k) add_unit<UNITS, E>(acc, v[k], split, fa, fb);
+          for (int k = 0; k < kAhead; ++k) sum.add(acc, v[k]);
         }
         for (; r < r1; r += sh.ty) {
           float v[E];
           load_unit<T, UNITS>(xu + static_cast<size_t>(r) * p.channels, v);
-          add_unit<UNITS, E>(acc, v, split, fa, fb);
+          sum.add(acc, v);
         }
+        sum.flush(acc);
       }
     }
-    reduce_groups<UNITS, E>(sh, acc, cg, ng, red,
-                            partial + (static_cast<size_t>(w) * p.chunks + blockIdx.x) * p.groups + g0);
-  }
+    reduce_groups<UNITS, E>(sh, acc, cg, ng, red, partial + (static_cast<size_t>(blockIdx.x) + w) * p.groups + g0);
+  });
 }
 
-// Statistics of groups [g0, g0 + ng) of a window, from its chunks' sums added
-// in chunk order, into `stat` (shared memory). All threads.
+// Statistics of groups [g0, g0 + ng) of window w, from its blocks' sums added
+// in a fixed order, into `stat` (shared memory). All threads.
 template <typename T>
 __device__ __forceinline__ void group_finish(const GroupNormParams& p, const GroupSum* partial, int w, int lo, int hi,
                                              int g0, int ng, GroupStat* stat) {
-  const int cg = p.channels / p.groups;
+  const int cg = p.channels / p.groups, first_block = lo / p.block, blocks = (hi - 1) / p.block - first_block + 1;
+  const int lane = threadIdx.x & 31;
+  const GroupSum* at = partial + (static_cast<size_t>(first_block) + w) * p.groups + g0;
   __syncthreads();  // stat has been read (previous window)
-  for (int g = threadIdx.x; g < ng; g += blockDim.x) {
-    GroupSum t{0.0, 0.0};
-    const GroupSum* at = partial + static_cast<size_t>(w) * p.chunks * p.groups + g0 + g;
-#pragma unroll 4
-    for (int c = 0; c < p.chunks; ++c) {
-      const GroupSum part = at[static_cast<size_t>(c) * p.groups];
-      t.s += part.s;
-      t.q += part.q;
+  // a warp per group, its lanes every 32nd block; or, for a few blocks, a thread per group
+  if (blocks <= 8) {
+    for (int g = threadIdx.x; g < ng; g += blockDim.x) {
+      GroupSum t{0.0, 0.0};
+      for (int c = 0; c < blocks; ++c) {
+        const GroupSum part = at[static_cast<size_t>(c) * p.groups + g];
+        t.s += part.s;
+        t.q += part.q;
+      }
+      stat[g] = group_stat(t, first_value<T>(p, lo, hi, g0, g, cg), static_cast<double>(hi - lo) * cg, p.eps);
     }
-    stat[g] = group_stat(t, first_value<T>(p, lo, hi, g0, g, cg), static_cast<double>(max(hi - lo, 1)) * cg, p.eps);
+  } else {
+    for (int g = threadIdx.x >> 5; g < ng; g += blockDim.x >> 5) {
+      const double first = first_value<T>(p, lo, hi, g0, g, cg);
+      GroupSum t{0.0, 0.0};
+      for (int c = lane; c < blocks; c += 32) {
+        const GroupSum part = at[static_cast<size_t>(c) * p.groups + g];
+        t.s += part.s;
+        t.q += part.q;
+      }
+      t.s = warp_sum_f64(t.s);
+      t.q = warp_sum_f64(t.q);
+      if (lane == 0) stat[g] = group_stat(t, first, static_cast<double>(hi - lo) * cg, p.eps);
+    }
   }
   __syncthreads();
 }
 
-// Normalise and activate the rows of one part of one window, one slab.
+// Normalise and activate one block of rows, one slab.
 template <typename T, int UNITS>
 __global__ void __launch_bounds__(kNormThreads)
     group_apply_kernel(const GroupNormParams p, const GroupSum* __restrict__ partial, T* __restrict__ y) {
@@ -377,46 +500,46 @@ __global__ void __launch_bounds__(kNormThreads)
   extern __shared__ GroupStat stat[];
   griddep_wait();
   griddep_launch();
-  const int cg = p.channels / p.groups, g0 = static_cast<int>(blockIdx.z) * p.slab, ng = min(p.slab, p.groups - g0);
+  const int cg = p.channels / p.groups, g0 = static_cast<int>(blockIdx.y) * p.slab, ng = min(p.slab, p.groups - g0);
   const SlabShape<E> sh(ng * cg);
-  for (int w = blockIdx.y; w < p.windows; w += gridDim.y) {
-    int lo, hi, r0, r1;
-    window_rows(p, w, &lo, &hi);
-    part_rows(lo, hi, blockIdx.x, gridDim.x, &r0, &r1);
+  const int b0 = static_cast<int>(blockIdx.x) * p.row_block;
+  const int b1 = static_cast<int>(min(static_cast<long long>(b0) + p.row_block, static_cast<long long>(p.rows)));
+  block_windows(p, b0, b1, [&](int w, int lo, int hi, int r0, int r1) {
     group_finish<T>(p, partial, w, lo, hi, g0, ng, stat);
-    if (sh.y >= sh.ty) continue;
-    for (int u = sh.x; u < sh.units; u += sh.tx) {
-      const int col = g0 * cg + u * E;
-      const UnitNorm<UNITS, E> norm(p, stat, u, cg, ng, col);
-      const T* const xu = static_cast<const T*>(p.x) + col;
-      T* const yu = y + col;
-      constexpr int kAhead = 4;
-      int r = r0 + sh.y;
-      for (; r + (kAhead - 1) * sh.ty < r1; r += kAhead * sh.ty) {
-        float v[kAhead][E];
+    if (sh.y < sh.ty) {
+      for (int u = sh.x; u < sh.units; u += sh.tx) {
+        const int col = g0 * cg + u * E;
+        const UnitNorm<UNITS, E> norm(p, stat, u, cg, ng, col);
+        const T* const xu = static_cast<const T*>(p.x) + col;
+        T* const yu = y + col;
+        constexpr int kAhead = 4;
+        int r = r0 + sh.y;
+        for (; r + (kAhead - 1) * sh.ty < r1; r += kAhead * sh.ty) {
+          float v[kAhead][E];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-          load_unit<T, UNITS>(xu + static_cast<size_t>(r + k * sh.ty) * p.channels, v[k]);
+          for (int k = 0; k < kAhead; ++k)
+            load_unit<T, UNITS>(xu + static_cast<size_t>(r + k * sh.ty) * p.channels, v[k]);
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          norm.apply(v[k], p.epi, p.round_out);
-          store_unit<T, UNITS>(yu + static_cast<size_t>(r + k * sh.ty) * p.channels, v[k]);
+          for (int k = 0; k < kAhead; ++k) {
+            norm.apply(v[k], p.epi, p.round_out);
+            store_unit<T, UNITS>(yu + static_cast<size_t>(r + k * sh.ty) * p.channels, v[k]);
+          }
+        }
+        for (; r < r1; r += sh.ty) {
+          float v[E];
+          load_unit<T, UNITS>(xu + static_cast<size_t>(r) * p.channels, v);
+          norm.apply(v, p.epi, p.round_out);
+          store_unit<T, UNITS>(yu + static_cast<size_t>(r) * p.channels, v);
         }
       }
-      for (; r < r1; r += sh.ty) {
-        float v[E];
-        load_unit<T, UNITS>(xu + static_cast<size_t>(r) * p.channels, v);
-        norm.apply(v, p.epi, p.round_out);
-        store_unit<T, UNITS>(yu + static_cast<size_t>(r) * p.channels, v);
-      }
     }
-  }
+  });
 }
 
-// Normalise, activate and quantise the rows of one part of one window: rows
-// whole, as their scale needs every channel.
+// Normalise, activate and quantise one block of rows: rows whole, as their
+// scale needs every channel.
 template <typename T, int CHUNKS, int WARPS, bool VEC>
-__global__ void __launch_bounds__(kRowThreads, 3)
+__global__ void __launch_bounds__(kRowThreads, 2)
     group_quantize_kernel(const GroupNormParams p, const GroupSum* __restrict__ partial, int8_t* __restrict__ q,
                           float* __restrict__ scale) {
   extern __shared__ GroupStat stat[];  // [groups], then their fp32 form
@@ -434,13 +557,12 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   src.fast = fast;
   src.group_width = p.channels / p.groups;
   src.whole = src.group_width % kChunk<T> == 0;
+  src.inv_width = 1.0f / src.group_width;
   src.epi = p.epi;
   src.top_b = cta_max_abs(p.b, p.channels, warp_top);
-  for (int w = blockIdx.y; w < p.windows; w += gridDim.y) {
-    int lo, hi, r0, r1;
-    window_rows(p, w, &lo, &hi);
-    part_rows(lo, hi, blockIdx.x, gridDim.x, &r0, &r1);
-    if (r0 >= r1) continue;  // the whole CTA
+  const int b0 = static_cast<int>(blockIdx.x) * p.row_block;
+  const int b1 = static_cast<int>(min(static_cast<long long>(b0) + p.row_block, static_cast<long long>(p.rows)));
+  block_windows(p, b0, b1, [&](int w, int lo, int hi, int r0, int r1) {
     group_finish<T>(p, partial, w, lo, hi, 0, p.groups, stat);
     for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
       const float m = static_cast<float>(stat[g].mean);
@@ -453,7 +575,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
       const float s = quantize_row<CHUNKS, WARPS>(src, p.channels, q + static_cast<size_t>(r) * p.channels, team);
       if (team.index() == 0) scale[r] = s;
     }
-  }
+  });
 }
 
 }  // namespace pq8

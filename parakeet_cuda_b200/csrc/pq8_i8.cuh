@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(kI8GemvThreads, 2) i8_gemv_kernel(const I8Para
 // As in pq8_gemm, the MMA's M dimension is 128 weight rows and its N dimension BN
 // tokens, so an epilogue thread owns one output channel (its scale and bias
 // stay in registers) and a warp's store covers 32 consecutive channels of one
-// token: coalesced for any n, without a staging tile. Both operands are
+// token: coalesced for any n, without a staging tile (tiles staged for TMA
+// stores measured no faster: 24000 x 1024 x 4096 to fp32 in 110 us against 104). Both operands are
 // K-major 128-byte rows, brought by TMA into 128-byte swizzled stages of 128
 // values of K; K past its end and rows past n or m arrive as zeros.
 //
@@ -205,8 +206,8 @@ __global__ void __launch_bounds__(kI8GemvThreads, 2) i8_gemv_kernel(const I8Para
 //
 // Two accumulators let the next tile's products run under a tile's epilogue.
 //
-// Warps: 0 TMA producer, 1 MMA issuer (and tensor-memory owner), 2 launch
-// control, 3 idle, 4-11 epilogue (two per lane quarter, half of the tokens each).
+// Warps: 0 and 2 TMA producers, 1 MMA issuer (and tensor-memory owner), 3
+// scheduler of the MMA issuer, 4 on: epilogue.
 __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
@@ -237,6 +238,14 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, in
       "l"(tmap), "r"(c0), "r"(c1), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_4d_pair(void* dst, const void* tmap, int c0, int c1, int c2, int c3,
+                                                 uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
+      "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
 // Adds 32-bit integers of this CTA's shared memory to those at `dst` in a CTA of the cluster.
 __device__ __forceinline__ void bulk_add_s2s_cluster(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
   asm volatile(
@@ -250,32 +259,40 @@ struct I8GemmParams {
   I8Params p;
   int n_tiles, m_tiles, k_blocks;  // 128-row weight tiles, BN-token tiles, 128-value K blocks
   int k_splits;
+  int glu_blocks;  // GLU: tmap_w is [n / 32][2][16][k], so that a tile's rows come in one load
 };
 
-template <int BN_, bool PAIR_, int STAGES_>
+template <int BN_, bool PAIR_>
 struct I8Cfg {
-  static constexpr int BN = BN_, STAGES = STAGES_, kCtas = PAIR_ ? 2 : 1;
+  static constexpr int STAGES = BN_ >= 128 ? 6 : 8;
+  static constexpr int kRelease = 2;  // K blocks per meeting of the scheduler and the MMA warp
+  static constexpr int BN = BN_, kCtas = PAIR_ ? 2 : 1;
   static constexpr bool PAIR = PAIR_;
   static constexpr int kTokens = BN / kCtas;  // token rows a CTA loads
   static constexpr int kABytes = 128 * 128, kBBytes = kTokens * 128, kStageBytes = kABytes + kBBytes;
-  static constexpr int E = BN >= 64 ? 32 : BN / 2;  // accumulator columns per tcgen05.ld
-  static constexpr int kChunks = BN / 2 / E;        // per epilogue half
-  static constexpr int kScaleOff = STAGES * kStageBytes;  // token scales of each epilogue warp's half tile
-  static constexpr int kBarOff = kScaleOff + 8 * (BN / 2) * 4;
+  // Epilogue: kGroups groups of 4 warps (one per TMEM lane quarter), each with
+  // kCols of the tile's tokens, E at a time. Sixteen warps for wide tiles: with
+  // eight, two to a scheduler, the epilogue's chains of dependent operations left
+  // most issue slots empty and it took longer than the products.
+  static constexpr int kGroups = BN >= 64 ? 4 : 2, kEpiWarps = 4 * kGroups, kCols = BN / kGroups;
+  static constexpr int E = kCols >= 16 ? 16 : 8;  // accumulator columns per tcgen05.ld
+  static constexpr int kChunks = kCols / E;
+  static constexpr int kScaleOff = STAGES * kStageBytes;  // token scales of each epilogue warp's part
+  static constexpr int kBarOff = kScaleOff + kEpiWarps * kCols * 4;
   static constexpr int kNumBars = 2 * STAGES + 4 + 2;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kSmemBytes = kMiscOff + 16 + 1024;
   static constexpr int kTmemCols = 2 * BN <= 32 ? 32 : 2 * BN <= 64 ? 64 : 2 * BN <= 128 ? 128 : 2 * BN <= 256 ? 256 : 512;
-  static constexpr int kThreads = 12 * 32;
-  static_assert(kTokens % 8 == 0 && BN % (PAIR ? 32 : 16) == 0 && BN <= 256 && (BN / 2) % E == 0, "tile shape");
+  static constexpr int kThreads = (4 + kEpiWarps) * 32;
+  static_assert(kTokens % 8 == 0 && BN % (PAIR ? 32 : 16) == 0 && BN <= 256 && kCols % E == 0, "tile shape");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory overflow");
+  static_assert(STAGES % 2 == 0, "the producers take stages in turn");
   static_assert(PAIR || BN * 128 * 4 <= STAGES * kStageBytes, "split K stages its sums in the ring");
 };
 
 template <int E>
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&v)[E]) {
-  if constexpr (E == 32) tmem_ld32(taddr, v);
-  else if constexpr (E == 16) tmem_ld16(taddr, v);
+  if constexpr (E == 16) tmem_ld16(taddr, v);
   else tmem_ld8(taddr, v);
 }
 
@@ -295,44 +312,62 @@ __device__ __forceinline__ void i8_epilogue(int epi, F&& f) {
 
 // The outputs of one channel for `cnt` <= E tokens (0: this lane stores
 // nothing) from their sums v, token scales sx, channel scale t and bias b;
-// `cols` elements apart at y. Every lane of the warp takes part (GLU: the gate
-// is the channel of the lane 16 further).
+// `cols` elements apart at y. Every lane of the warp takes part. GLU: lanes
+// 0-15 have a value channel and lanes 16-31 its gate; of each two tokens
+// the lower lane finishes the first and the upper lane the second.
 template <typename T, int E, int EPI>
 __device__ __forceinline__ void i8_finish(const uint32_t (&v)[E], const T (&rv)[E], const float* sx, float t, float b,
                                           float alpha, T* y, int cols, int cnt) {
-  T out[E];
+  constexpr bool kGlu = EPI == PQ8_EPI_GLU;
+  constexpr int N = kGlu ? E / 2 : E;  // outputs of this lane
+  const bool upper = (threadIdx.x & 16) != 0;
+  const f32x2 t2 = pack2(t, t), b2 = pack2(b, b);
+  float out[N];
+  float a_prev = 0.0f, g_prev = 0.0f;  // GLU: the first of two outputs' value and gate
 #pragma unroll
-  for (int j = 0; j < E; j += 4) {
-    const float4 s4 = *reinterpret_cast<const float4*>(sx + j);
-    const float s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float z = i8_scaled(static_cast<int>(v[j + i]), s[i], t, b);
-      if constexpr (EPI == PQ8_EPI_RESIDUAL) z = fmaf(alpha, z, to_f32(rv[j + i]));
-      if constexpr (EPI == PQ8_EPI_SILU) z = __fdividef(z, 1.0f + __expf(-z));
-      if constexpr (EPI == PQ8_EPI_RELU) z = fmaxf(z, 0.0f);
-      if constexpr (EPI == PQ8_EPI_GLU) {
-        const float gate = __shfl_down_sync(0xffffffffu, z, 16);
-        z = __fdividef(z, 1.0f + __expf(-gate));
+  for (int j = 0; j < E; j += 2) {
+    const f32x2 s = *reinterpret_cast<const f32x2*>(sx + j);
+    f32x2 z = fma2(mul2(pack2(static_cast<float>(static_cast<int>(v[j])), static_cast<float>(static_cast<int>(v[j + 1]))), s), t2, b2);
+    if constexpr (kGlu) {
+      float z0, z1;
+      unpack2(z, &z0, &z1);
+      const float other = __shfl_xor_sync(0xffffffffu, upper ? z0 : z1, 16);
+      const float a = upper ? other : z0, gate = upper ? z1 : other;
+      if (j % 4 == 0) {
+        a_prev = a;
+        g_prev = gate;
+      } else {
+        unpack2(mul2(pack2(a_prev, a), sigmoid2(pack2(g_prev, gate))), &out[j / 2 - 1], &out[j / 2]);
       }
-      out[j + i] = from_f32<T>(z);
+    } else {
+      if constexpr (EPI == PQ8_EPI_RESIDUAL) z = fma2(pack2(alpha, alpha), z, pack2(to_f32(rv[j]), to_f32(rv[j + 1])));
+      if constexpr (EPI == PQ8_EPI_SILU) z = mul2(z, sigmoid2(z));
+      unpack2(z, &out[j], &out[j + 1]);
+      if constexpr (EPI == PQ8_EPI_RELU) {
+        out[j] = fmaxf(out[j], 0.0f);
+        out[j + 1] = fmaxf(out[j + 1], 0.0f);
+      }
     }
   }
+  constexpr int kStep = E / N;
+  T* const y0 = y + (kGlu && upper ? cols : 0);
+  const int mine = kGlu && upper ? cnt - 1 : cnt;  // GLU: tokens 1, 3, ... of the upper lanes
   if (cnt == E) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) y[static_cast<size_t>(j) * cols] = out[j];
+    for (int j = 0; j < N; ++j) y0[static_cast<size_t>(j * kStep) * cols] = from_f32<T>(out[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < E; ++j)
-      if (j < cnt) y[static_cast<size_t>(j) * cols] = out[j];
+    for (int j = 0; j < N; ++j)
+      if (j * kStep < mine) y0[static_cast<size_t>(j * kStep) * cols] = from_f32<T>(out[j]);
   }
 }
 
-template <typename T, int BN, bool PAIR, int STAGES>
-__global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
+template <typename T, int BN, bool PAIR>
+__global__ void __launch_bounds__(I8Cfg<BN, PAIR>::kThreads, 1)
     i8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                    const __grid_constant__ I8GemmParams g) {
-  using C = I8Cfg<BN, PAIR, STAGES>;
+  using C = I8Cfg<BN, PAIR>;
+  constexpr int STAGES = C::STAGES;
   const I8Params& p = g.p;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -360,7 +395,7 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8 * C::kCtas);  // one arrival per epilogue warp
+      mbar_init(&acc_empty[a], C::kEpiWarps * C::kCtas);  // one arrival per epilogue warp
     }
     mbar_init(drain, 1);
     mbar_init(red_full, 1);
@@ -395,17 +430,23 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
   const int per_split = (g.k_blocks + S - 1) / S;
   const int kb0 = my_split * per_split, kb1 = min(kb0 + per_split, g.k_blocks);
 
-  if (warp == 0) {
-    // ------------------------------------------------------------- producer
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------------ producers
+    // Two, taking K blocks (and so stages) in turn: a thread that has issued TMA
+    // loads takes a few hundred cycles until its next barrier wait is answered.
     if (lane == 0) {
+      const uint32_t me = warp >> 1;
       griddep_wait();
+      if (me == 1) griddep_launch();
       const uint32_t full_at = PAIR ? map_to_rank(full, 0) : smem_addr(full);
-      uint32_t issued = 0;
+      uint32_t it = 0;  // K blocks so far, of both producers
       Ring<STAGES> ring;
+      ring.advance(me);
       for (int tile = tile0; tile < num_tiles; tile += tile_step) {
         const int unit = tile % n_units, token0 = (tile / n_units) * BN + static_cast<int>(rank) * C::kTokens;
         const int n_tile = unit * C::kCtas + static_cast<int>(rank);
-        for (int kb = kb0; kb < kb1; ++kb, ++issued, ring.advance(1)) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          if ((it & 1) != me) continue;
           if (!mbar_wait(&empty[ring.idx], ring.phase ^ 1u, abort_flag, status)) goto loads_done;
           uint8_t* a = smem + ring.idx * C::kStageBytes;
           const uint32_t bar = full_at + ring.idx * 8;
@@ -416,25 +457,56 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
           };
           if (glu) {
             // 16 rows of the first half, then the 16 gate rows of the same channels, four times
+            if (g.glu_blocks) {
+              if constexpr (PAIR) tma_load_4d_pair(a, &tmap_w, kb * 128, 0, 0, n_tile * 4, bar);
+              else tma_load_4d(a, &tmap_w, kb * 128, 0, 0, n_tile * 4, &full[ring.idx]);
+            } else {
 #pragma unroll 1
-            for (int i = 0; i < 8; ++i)
-              load(a + i * 2048, &tmap_w, ((i & 1) ? p.n / 2 : 0) + n_tile * 64 + (i >> 1) * 16);
+              for (int i = 0; i < 8; ++i)
+                load(a + i * 2048, &tmap_w, ((i & 1) ? p.n / 2 : 0) + n_tile * 64 + (i >> 1) * 16);
+            }
           } else {
             load(a, &tmap_w, n_tile * 128);
           }
           load(a + C::kABytes, &tmap_x, token0);
+          ring.advance(2);
         }
       }
     loads_done:
       // no copy may land in the shared memory of a CTA that has gone (the
       // leader's barriers count the peer's too, and the pair leaves together)
       if (leader)
-        for (uint32_t j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j)
-          mbar_drain(&full[j % STAGES], (j / STAGES) & 1);
+        for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
+          if ((j & 1) == me) mbar_drain(&full[j % STAGES], (j / STAGES) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ------------------------------------------------------------- scheduler
+    // Waits on every barrier the products depend on and releases the MMA warp
+    // through a named barrier: a shared-memory access by the warp that
+    // issues tcgen05.mma is held behind the products it has queued, so its own
+    // waits would drain the tensor pipe at every K block (128 x 16384 x 1024 in
+    // tiles of 32: 39 us with the MMA warp waiting for itself, 35 so). Both warps meet the same
+    // number of times; the barrier carries the flag to stop.
+    if (leader) {
+      bool bad = false;
+      int local = 0;
+      Ring<STAGES> ring;
+      for (int tile = tile0; tile < num_tiles && !bad; tile += tile_step, ++local) {
+        if (lane == 0) bad = !mbar_wait(&acc_empty[local & 1], ((local >> 1) & 1) ^ 1, abort_flag, status);
+        for (int kb = kb0; kb < kb1 && !bad; kb += C::kRelease) {
+          const int n = min(C::kRelease, kb1 - kb);
+          if (lane == 0)
+            for (int b = 0; b < n && !bad; ++b, ring.advance(1))
+              bad = !mbar_wait(&full[ring.idx], ring.phase, abort_flag, status);
+          bad = __shfl_sync(0xffffffffu, bad, 0);
+          bad = rendezvous_or(1, bad);
+        }
+      }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (leader && lane == 0) {
+    if (leader) {
       constexpr uint32_t idesc = idesc_i8(128 * C::kCtas, BN);
       const uint64_t desc0 = smem_desc_sw128(smem_addr(smem));
       bool stop = false, issued = false;
@@ -442,42 +514,45 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
       Ring<STAGES> ring;
       for (int tile = tile0; tile < num_tiles && !stop; tile += tile_step, ++local) {
         const int acc = local & 1;
-        if (!mbar_wait(&acc_empty[acc], ((local >> 1) & 1) ^ 1, abort_flag, status)) break;
-        tc_fence_after();
         const uint32_t d = tmem + acc * BN;
-        for (int kb = kb0; kb < kb1; ++kb, ring.advance(1)) {
-          if (!mbar_wait(&full[ring.idx], ring.phase, abort_flag, status)) {
+        for (int kb = kb0; kb < kb1; kb += C::kRelease) {
+          const int n = min(C::kRelease, kb1 - kb);
+          if (rendezvous_or(1, false)) {  // the scheduler gave up
             stop = true;
             break;
           }
           tc_fence_after();
-          const uint64_t ad = desc0 + ring.idx * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
+          if (lane == 0) {
+            for (int b = 0; b < n; ++b, ring.advance(1)) {
+              const uint64_t ad = desc0 + ring.idx * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma_i8<PAIR>(d, ad + 2 * j, bd + 2 * j, idesc, (kb > kb0 || j > 0) ? 1u : 0u);
+              for (int j = 0; j < 4; ++j)
+                mma_i8<PAIR>(d, ad + 2 * j, bd + 2 * j, idesc, (kb + b > kb0 || j > 0) ? 1u : 0u);
+              if constexpr (PAIR) mma_commit_pair(&empty[ring.idx], 0x3);
+              else mma_commit(&empty[ring.idx]);
+            }
+            if (kb + n == kb1) {
+              if constexpr (PAIR) mma_commit_pair(&acc_full[acc], 0x3);
+              else mma_commit(&acc_full[acc]);
+            }
+          }
+          __syncwarp();
           issued = true;
-          if constexpr (PAIR) mma_commit_pair(&empty[ring.idx], 0x3);
-          else mma_commit(&empty[ring.idx]);
         }
-        if (stop) break;
-        if constexpr (PAIR) mma_commit_pair(&acc_full[acc], 0x3);
-        else mma_commit(&acc_full[acc]);
       }
-      if (issued && *abort_flag) {  // the products under way end before the CTA is torn down
+      if (stop && issued && lane == 0) {  // the products under way end before the CTA is torn down
         if constexpr (PAIR) mma_commit_pair(drain, 0x1);
         else mma_commit(drain);
         mbar_drain(drain, 0);
       }
     }
     __syncwarp();
-  } else if (warp == 2) {
-    griddep_wait();
-    griddep_launch();
   } else if (warp >= 4) {
     // -------------------------------------------------------------- epilogue
     constexpr int E = C::E;
-    const int q = warp & 3, half = (warp - 4) >> 2, r = q * 32 + lane;
+    const int q = warp & 3, group = (warp - 4) >> 2, r = q * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
-    float* sx = reinterpret_cast<float*>(smem + C::kScaleOff) + (warp - 4) * (BN / 2);
+    float* sx = reinterpret_cast<float*>(smem + C::kScaleOff) + (warp - 4) * C::kCols;
     const uint32_t acc_empty_at = PAIR ? map_to_rank(acc_empty, 0) : smem_addr(acc_empty);
     bool published = false;
     griddep_wait();
@@ -490,7 +565,6 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
       const int col = glu ? n_tile * 64 + q * 16 + (lane & 15) : n_tile * 128 + r;
       const int row = glu && lane >= 16 ? p.n / 2 + col : col;
       const bool valid = col < p.out_cols;
-      const bool stores = valid && (!glu || lane < 16);
       const float t = valid ? __ldg(p.w_scale + row) : 0.0f;
       const float b = (valid && p.bias != nullptr) ? __ldg(p.bias + row) : 0.0f;
       T* const y = static_cast<T*>(p.y) + col;
@@ -501,26 +575,26 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
       auto finish = [&](const uint32_t(&v)[E], const T(&rv)[E], const float* sx, int m0, int cnt) {
         T* const yp = y + static_cast<size_t>(m0) * cols;
         i8_epilogue(p.epi, [&](auto epi) {
-          i8_finish<T, E, decltype(epi)::value>(v, rv, sx, t, b, p.alpha, yp, cols, stores ? cnt : 0);
+          i8_finish<T, E, decltype(epi)::value>(v, rv, sx, t, b, p.alpha, yp, cols, valid ? cnt : 0);
         });
       };
       auto load_resid = [&](T(&rv)[E], int m0, int cnt) {
         if (p.epi == PQ8_EPI_RESIDUAL) {
 #pragma unroll
-          for (int j = 0; j < E; ++j) rv[j] = (stores && j < cnt) ? res[static_cast<size_t>(m0 + j) * cols] : from_f32<T>(0.0f);
+          for (int j = 0; j < E; ++j) rv[j] = (valid && j < cnt) ? res[static_cast<size_t>(m0 + j) * cols] : from_f32<T>(0.0f);
         }
       };
-      // the scales of up to BN / 2 tokens from m0 on, for this warp
+      // the scales of up to kCols tokens from m0 on, for this warp
       auto load_scales = [&](int m0) {
         __syncwarp();  // the previous tile's have been read
 #pragma unroll
-        for (int i = 0; i < BN / 2; i += 32)
-          if (i + lane < BN / 2) sx[i + lane] = m0 + i + lane < p.m ? __ldg(p.x_scale + m0 + i + lane) : 0.0f;
+        for (int i = 0; i < C::kCols; i += 32)
+          if (i + lane < C::kCols) sx[i + lane] = m0 + i + lane < p.m ? __ldg(p.x_scale + m0 + i + lane) : 0.0f;
         __syncwarp();
       };
       T rv[E];
       if (!split) {
-        const int first = token0 + half * (BN / 2);
+        const int first = token0 + group * C::kCols;
         load_scales(first);
         load_resid(rv, first, min(E, p.m - first));
         if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag, status)) break;
@@ -529,7 +603,7 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
         for (int cc = 0; cc < C::kChunks; ++cc) {
           const int m0 = first + cc * E, cnt = min(E, p.m - m0);
           uint32_t v[E];
-          tmem_ld_cols<E>(tmem + lane_base + acc * BN + half * (BN / 2) + cc * E, v);
+          tmem_ld_cols<E>(tmem + lane_base + acc * BN + group * C::kCols + cc * E, v);
           tmem_wait_ld();
           if (cc + 1 == C::kChunks) {
             tc_fence_before();
@@ -552,7 +626,7 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
         tc_fence_after();
 #pragma unroll 1
         for (int cc = 0; cc < C::kChunks; ++cc) {
-          const int c0 = half * (BN / 2) + cc * E;
+          const int c0 = group * C::kCols + cc * E;
           uint32_t v[E];
           tmem_ld_cols<E>(tmem + lane_base + c0, v);
           tmem_wait_ld();
@@ -573,7 +647,7 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR, STAGES>::kThreads, 1)
           bulk_add_s2s_cluster(map_to_rank(src, d), src, static_cast<uint32_t>(R * 512), map_to_rank(red_full, d));
         }
         __syncwarp();
-        const int rows = R / 2, off = my_split * R + half * rows;
+        const int rows = R / C::kGroups, off = my_split * R + group * rows;
         const int cnt_all = min(rows, p.m - token0 - off);
         load_scales(token0 + off);
         if (!mbar_wait(red_full, 0, abort_flag, status)) break;

@@ -94,6 +94,47 @@ __device__ __forceinline__ float cta_max_abs(const float* b, int n, float* smem 
   return top;
 }
 
+// Two fp32 values per instruction (packed operands of sm_100).
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Sigmoids of two values. 1 / (1 + e^-z) takes an exponential and a reciprocal from
+// the special-function unit, which bounds epilogues with few other operations;
+// here the two share one reciprocal: 1 / d0 = d1 / (d0 d1). The exponent is
+// capped at 63 so that the product stays in range; below z = -43.7 the
+// result is 2^-63 instead of e^z, an absolute error under 2^-63.
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 z) {
+  float e0, e1, r;
+  unpack2(mul2(z, pack2(-1.44269504f, -1.44269504f)), &e0, &e1);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(e0, 63.0f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(e1, 63.0f)));
+  unpack2(add2(pack2(e0, e1), pack2(1.0f, 1.0f)), &e0, &e1);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e0 * e1));
+  return mul2(pack2(r, r), pack2(e1, e0));
+}
+
 template <typename T, int E>
 __device__ __forceinline__ void store_chunk(T* p, bool vec, const float (&v)[E]) {
   if (vec) {
@@ -113,10 +154,12 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// Of values >= 0, whose bit patterns are ordered as they are: the high words
+// first, then the low words of the lanes that have the highest.
 __device__ __forceinline__ double warp_max_f64(double v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  const unsigned hi = static_cast<unsigned>(__double2hiint(v)), top = __reduce_max_sync(0xffffffffu, hi);
+  const unsigned lo = __reduce_max_sync(0xffffffffu, hi == top ? static_cast<unsigned>(__double2loint(v)) : 0u);
+  return __hiloint2double(static_cast<int>(top), static_cast<int>(lo));
 }
 
 // Reductions over the WARPS warps that share a row. Sums are added in a fixed
@@ -270,24 +313,37 @@ struct GroupNormSource {
   const GroupStat* stat;  // [groups], shared memory
   const float4* fast;     // [groups], shared memory: mean's high and low part, 1 / deviation in fp32
   int group_width;
+  float inv_width;        // 1 / group_width
   bool whole;             // a chunk lies within one group
   int epi;
   float top_b;  // max|b|
+  // col / group_width for columns below 2^20: the quotient of col + 1/2 is at
+  // least 1 / (2 group_width) from a whole number, more than the product's error
+  __device__ __forceinline__ int group(int col) const {
+    return static_cast<int>((static_cast<float>(col) + 0.5f) * inv_width);
+  }
   __device__ __forceinline__ void raw(int c, float (&v)[E]) const { load_chunk<T, E>(x + c * E, VEC, v); }
   __device__ __forceinline__ void value(int c, float (&v)[E]) const {
     float g[E], h[E];
     load_params<E>(w + c * E, VEC, g);
     load_params<E>(b + c * E, VEC, h);
     if (whole) {
-      const float4 f = fast[c * E / group_width];
+      const float4 f = fast[group(c * E)];
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = act_f32(fmaf(((v[i] - f.x) - f.y) * f.z, g[i], h[i]), epi);
+      for (int i = 0; i < E; ++i) v[i] = fmaf(((v[i] - f.x) - f.y) * f.z, g[i], h[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const float4 f = fast[(c * E + i) / group_width];
-        v[i] = act_f32(fmaf(((v[i] - f.x) - f.y) * f.z, g[i], h[i]), epi);
+        const float4 f = fast[group(c * E + i)];
+        v[i] = fmaf(((v[i] - f.x) - f.y) * f.z, g[i], h[i]);
       }
+    }
+    if (epi == PQ8_EPI_SILU) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = act_f32(v[i], PQ8_EPI_SILU);
+    } else if (epi == PQ8_EPI_RELU) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = act_f32(v[i], PQ8_EPI_RELU);
     }
   }
   __device__ __forceinline__ double exact(int col) const {

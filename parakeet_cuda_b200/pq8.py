@@ -105,7 +105,7 @@ SIGNATURES = {
     'pq8_gemm_i8': ([_P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _P], _I),
     'pq8_linear_i8_workspace_size': ([_I, _I, C.POINTER(_SZ)], _I),
     'pq8_linear_i8': ([_P, _P, _P, _I, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _P, _SZ, _P], _I),
-    'pq8_group_norm_workspace_size': ([_I, _I, _I, _I, _I, _I, _I, C.POINTER(_SZ)], _I),
+    'pq8_group_norm_workspace_size': ([_I, _I, _I, _I, _I, _I, _I, _I, C.POINTER(_SZ)], _I),
     'pq8_group_norm': ([_P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _D, _I, _I, _P, _SZ, _P], _I),
     'pq8_group_norm_quantize': ([_P, _I, _P, _P, _P, _P, _I, _I, _P, _I, _I, _D, _I, _P, _SZ, _P], _I),
 }
@@ -194,9 +194,9 @@ class Library:
         return out.value
 
     def group_norm_workspace_size(self, kind: int, rows: int, windows: int, channels: int, groups: int,
-                                  quantize: bool = False, aligned16: bool = True) -> int:
+                                  ragged: bool = False, quantize: bool = False, aligned16: bool = True) -> int:
         out = _SZ()
-        self.call('pq8_group_norm_workspace_size', kind, rows, windows, channels, groups, quantize, aligned16,
+        self.call('pq8_group_norm_workspace_size', kind, rows, windows, channels, groups, ragged, quantize, aligned16,
                   C.byref(out))
         return out.value
 

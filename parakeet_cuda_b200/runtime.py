@@ -458,7 +458,8 @@ class Runtime:
             y = out.data_ptr()
         else:
             y = self._check(out, 'out', x.dtype, x.shape)
-        need = self.lib.group_norm_workspace_size(kind, rows, windows, channels, groups, False, not (at[0] | y) & 15)
+        need = self.lib.group_norm_workspace_size(kind, rows, windows, channels, groups, off is not None, False,
+                                                  not (at[0] | y) & 15)
         scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._enqueue('pq8_group_norm', at[0], kind, at[1], at[2], y, rows, windows, off, channels, groups, eps,
                       epilogue, flags, _ptr(scratch), need)
@@ -471,7 +472,7 @@ class Runtime:
         rows, channels, kind, at, off = self._check_group_norm(x, weight, bias, windows, offsets)
         out = QuantizedRows(torch.empty(rows, channels, dtype=torch.int8, device=self.device),
                             torch.empty(rows, dtype=torch.float32, device=self.device))
-        need = self.lib.group_norm_workspace_size(kind, rows, windows, channels, groups, True,
+        need = self.lib.group_norm_workspace_size(kind, rows, windows, channels, groups, off is not None, True,
                                                   not (at[0] | at[1] | at[2]) & 15)
         scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._enqueue('pq8_group_norm_quantize', at[0], kind, at[1], at[2], out.q_ptr, out.scale_ptr, rows, windows,

@@ -1,9 +1,17 @@
 """GPU parity of the channels-last group norm against the 64-bit oracle.
 
-Tolerance: mean and variance are fp64; the deviation, the multiplication by 1 / sqrt(var + eps)
-(itself rounded to fp32) and the multiply-add with weight and bias round under 6 times relative to
-|y| + |b|, ReLU and SiLU pass an error on with a slope of at most 1.1, SiLU adds under
-8 x 2^-24 of its result; then half a step of the output's type.
+Tolerance, with U = 2^-24 and everything in units of the group's deviation. Rounding after the
+statistics: the deviation from the mean, the scale w / deviation, the remainder of the bias and the
+multiply-add round under 6 U (|z| + |b|) together. Statistics: a column's differences from its first
+value of up to 32 rows, |d| <= D, are summed in fp32. The differences round by U D, and the k-th of m
+additions by U k D, so a run's sum is off by at most U D (m + m (m + 1) / 2) and its mean by
+U D (1 + (m + 1) / 2) <= 18 U D (m = 32); of the squares likewise, the difference's rounding counting
+twice and the product's once: the mean square by U D^2 (3 + (m + 1) / 2) <= 20 U D^2. (All above the
+runs is fp64.) The shift by the run's reference moves the mean's error R into the mean square by 2 R D.
+So the mean is off by 18 U D and the variance by 56 U D^2, 1 / sqrt(var) by half that, relative:
+|dz| <= |w| 18 U D + (|z| + |b|) 28 U D^2, D <= twice the largest |x - mean| of window and group. (Rounding
+errors have either sign; the sums' true error is far below.) ReLU and SiLU pass an error on with a
+slope of at most 1.1, SiLU adds under 8 U of its result; then half a step of the output's type.
 """
 import numpy as np
 import pytest
@@ -42,14 +50,29 @@ def inputs(seed, rows, channels, dtype, offset=0.5):
     return dev(x.astype(np.float32), dtype), dev(w.astype(np.float32)), dev(b.astype(np.float32))
 
 
+def spread(x, groups, bounds):
+    """D of the module's tolerance for every value: twice the largest |x - mean| / sqrt(var + eps)."""
+    c = x.shape[1]
+    one, zero = np.ones(c), np.zeros(c)
+    z = np.abs(oi.group_norm(x, one, zero, groups, bounds))
+    out = np.zeros_like(z)
+    for lo, hi in zip(bounds[:-1], bounds[1:]):
+        if hi > lo:
+            blk = z[lo:hi].reshape(hi - lo, groups, c // groups)
+            out[lo:hi] = (0 * blk + 2 * blk.max(axis=(0, 2), keepdims=True)).reshape(hi - lo, c)
+    return out
+
+
 def check(got, x, w, b, groups, bounds, act, extra=0.0):
     z = oi.group_norm(f64(x), f64(w), f64(b), groups, bounds)
+    far = spread(f64(x), groups, bounds)
     y = oi.act(z, act)
     inside = np.zeros(len(z), bool)
     for lo, hi in zip(bounds[:-1], bounds[1:]):
         inside[lo:hi] = True
-    g, y, z = f64(got)[inside], y[inside], z[inside]
-    err = 1.1 * 6 * U * (np.abs(z) + np.abs(f64(b))) + 8 * U * np.abs(y)
+    g, y, z, far = f64(got)[inside], y[inside], z[inside], far[inside]
+    size = np.abs(z) + np.abs(f64(b))
+    err = 1.1 * U * (6 * size + 18 * far * np.abs(f64(w)) + 28 * far ** 2 * size) + 8 * U * np.abs(y)
     fi = torch.finfo(got.dtype)
     bound = err + fi.eps / 2 * (np.abs(y) + err) + fi.tiny * fi.eps + extra * np.abs(y) + 1e-37
     assert np.isfinite(g).all()
@@ -104,19 +127,21 @@ def test_group_norm_rows_outside_do_not_matter(rt):
 
 
 def test_group_norm_offsets_outside_the_rows(rt):
-    """Offsets beyond the rows, negative or falling are held inside: nothing outside x and y is touched.
-    These give windows [0, 10), none, [4, 32) and none: rows 4 to 9 are two windows' (either may have
-    written last), the others have one window each."""
-    x, w, b = inputs(6, 32, 64, torch.float32)
-    guard = torch.full((3, 32, 64), 5.0, device='cuda')
-    off = torch.tensor([-7, 10, 4, 1000, 2 ** 31 - 1], dtype=torch.int32, device='cuda')
-    rt.group_norm(x, w, b, 4, windows=4, offsets=off, out=guard[1])
-    assert (guard[0] == 5).all() and (guard[2] == 5).all()
-    first, third = guard[1].clone(), guard[1].clone()
-    first[4:10] = torch.nan_to_num(dev(oi.group_norm(f64(x), f64(w), f64(b), 4, [0, 10]).astype(np.float32)))[4:10]
-    check(first[:10], x[:10], w, b, 4, [0, 10], 'none')
-    third[4:10] = dev(oi.group_norm(f64(x), f64(w), f64(b), 4, [4, 32]).astype(np.float32))[4:10]
-    check(third[4:], x[4:], w, b, 4, [0, 28], 'none')
+    """Offsets beyond the rows are held inside; falling ones leave the values of their rows open, but nothing
+    outside the output is touched."""
+    for channels, groups in ((64, 4), (1000, 8), (35, 5)):  # one launch, units that straddle groups, single columns
+        x, w, b = inputs(6, 32, channels, torch.float32)
+        guard = torch.full((3, 32, channels), 5.0, device='cuda')
+        off = torch.tensor([-7, 10, 10, 1000, 2 ** 31 - 1], dtype=torch.int32, device='cuda')
+        rt.group_norm(x, w, b, groups, windows=4, offsets=off, out=guard[1])
+        check(guard[1], x, w, b, groups, [0, 10, 10, 32], 'none')
+        for bad in ([20, 10, 4, 1000, -5], [2 ** 31 - 1, 0, 32, 16, 31], [-2 ** 31, -1, 40, 3, 3]):
+            rt.group_norm(x, w, b, groups, windows=4, out=guard[1],
+                          offsets=torch.tensor(bad, dtype=torch.int32, device='cuda'))
+            if channels % 16 == 0:
+                rt.group_norm_quantize(x, w, b, groups, windows=4,
+                                       offsets=torch.tensor(bad, dtype=torch.int32, device='cuda'))
+        assert (guard[0] == 5).all() and (guard[2] == 5).all()
 
 
 def test_group_norm_large_offset_and_long_window(rt):

@@ -134,7 +134,7 @@ def test_group_norm_refusals(lib):
     for bad in ((0, 12, 3, 64, 5), (3, 12, 3, 64, 4), (0, -1, 3, 64, 4)):
         with pytest.raises(pq8.PQ8Error):
             lib.group_norm_workspace_size(*bad)
-    assert code(lib, 'pq8_group_norm_workspace_size', 0, 12, 3, 64, 4, 0, 1, None) == pq8.ERR_INVALID_ARGUMENT
+    assert code(lib, 'pq8_group_norm_workspace_size', 0, 12, 3, 64, 4, 0, 0, 1, None) == pq8.ERR_INVALID_ARGUMENT
     assert code(lib, 'pq8_group_norm_quantize', X, 0, W, B, Q, S, 12, 3, None, 60, 4, 1e-5, 0, WS, BIG,
                 None) == pq8.ERR_UNSUPPORTED_SHAPE
     assert code(lib, 'pq8_group_norm_quantize', X, 0, W, B, Q, None, 12, 3, None, 64, 4, 1e-5, 0, WS, BIG,
