@@ -2543,7 +2543,8 @@ struct GroupNormPlan {
   int hold;           // one launch: rows a CTA holds
   size_t smem;        // one launch
   int block, row_block;  // two launches: rows a CTA takes, for the sums and in the second launch
-  size_t total;       // workspace
+  // workspace; quantised form: one launch's values and statistics, or the sums; and max|b|
+  size_t stat, top_b, total;
 };
 
 constexpr size_t kNormMaxSmem = size_t(200) << 10;
@@ -2576,7 +2577,7 @@ GroupNormPlan plan_group_norm(int size, bool vec, int rows, int windows, bool ra
   const long long units = static_cast<long long>(std::max(windows, 1)) * g.slabs;
   const int t = std::max(1, (rows + std::max(windows, 1) - 1) / std::max(windows, 1));
   const size_t row_bytes = static_cast<size_t>(g.slab) * cg * size;
-  if (!quantize && g.units != kScalar && windows <= 65535) {
+  if (g.units != kScalar && windows <= 65535) {
     // One launch: the smallest cluster that holds an average window at four
     // CTAs an SM, and that gives every SM a CTA; at most 8 CTAs. Windows of
     // unequal lengths take it only where its CTAs are many enough to even out.
@@ -2590,6 +2591,11 @@ GroupNormPlan plan_group_norm(int size, bool vec, int rows, int windows, bool ra
       g.parts = parts;
       g.hold = per;
       g.smem = per * row_bytes + tables;
+      if (quantize) {
+        g.stat = round256(static_cast<size_t>(rows) * channels * sizeof(float));
+        g.top_b = g.stat + round256(static_cast<size_t>(windows) * groups * sizeof(GroupStat));
+        g.total = g.top_b + 256;
+      }
       return g;
     }
   }
@@ -2600,7 +2606,8 @@ GroupNormPlan plan_group_norm(int size, bool vec, int rows, int windows, bool ra
   };
   g.block = block(g.slabs, 4 * sms, 16);
   g.row_block = quantize ? block(1, 4 * sms, 8) : g.block;
-  g.total = round256(sizeof(GroupSum) * (static_cast<size_t>((rows + g.block - 1) / g.block) + windows) * groups);
+  g.top_b = round256(sizeof(GroupSum) * (static_cast<size_t>((rows + g.block - 1) / g.block) + windows) * groups);
+  g.total = g.top_b + 256;
   return g;
 }
 
@@ -2668,9 +2675,10 @@ auto with_units(int units, F&& f) {
   return units == kWhole ? f(UnitsTag<kWhole>{}) : units == kStraddle ? f(UnitsTag<kStraddle>{}) : f(UnitsTag<kScalar>{});
 }
 
-template <typename T, int UNITS>
-cudaError_t launch_group_norm_one(const GroupNormPlan& g, const GroupNormParams& p, T* y, cudaStream_t st) {
-  auto kernel = group_norm_kernel<T, UNITS>;
+template <typename T, int UNITS, bool QUANT>
+cudaError_t launch_group_norm_one(const GroupNormPlan& g, const GroupNormParams& p,
+                                  std::conditional_t<QUANT, float, T>* y, GroupNormExtra extra, cudaStream_t st) {
+  auto kernel = group_norm_kernel<T, UNITS, QUANT>;
   static bool attr_set[kMaxDevices];
   const cudaError_t ea = allow_smem(kernel, static_cast<int>(kNormMaxSmem), attr_set);
   if (ea != cudaSuccess) return ea;
@@ -2688,14 +2696,16 @@ cudaError_t launch_group_norm_one(const GroupNormPlan& g, const GroupNormParams&
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g.parts > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p, y);
+  return cudaLaunchKernelEx(&cfg, kernel, p, y, extra);
 }
 
 template <typename T, bool EXACT>
-cudaError_t launch_group_stats(const GroupNormPlan& g, const GroupNormParams& p, GroupSum* partial, cudaStream_t st) {
+cudaError_t launch_group_stats(const GroupNormPlan& g, const GroupNormParams& p, void* workspace, cudaStream_t st) {
+  GroupSum* partial = static_cast<GroupSum*>(workspace);
+  float* top_b = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + g.top_b);
   const dim3 grid((p.rows + g.block - 1) / g.block, g.slabs);
   return with_units(g.units, [&](auto u) {
-    return launch_pdl(group_stats_kernel<T, decltype(u)::value, EXACT>, grid, dim3(kNormThreads), 0, st, p, partial);
+    return launch_pdl(group_stats_kernel<T, decltype(u)::value, EXACT>, grid, dim3(kNormThreads), 0, st, p, partial, top_b);
   });
 }
 
@@ -2735,10 +2745,11 @@ extern "C" int pq8_group_norm(const void* x, int type, const float* w, const flo
     GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
     p.round_out = (flags & PQ8_FLAG_OUT_TF32) ? 1 : 0;
     if (g.parts > 0)
-      return g.units == kWhole ? launch_group_norm_one<T, kWhole>(g, p, static_cast<T*>(y), st)
-                               : launch_group_norm_one<T, kStraddle>(g, p, static_cast<T*>(y), st);
+      return g.units == kWhole
+                 ? launch_group_norm_one<T, kWhole, false>(g, p, static_cast<T*>(y), GroupNormExtra{}, st)
+                 : launch_group_norm_one<T, kStraddle, false>(g, p, static_cast<T*>(y), GroupNormExtra{}, st);
     GroupSum* partial = static_cast<GroupSum*>(workspace);
-    const cudaError_t err = launch_group_stats<T, false>(g, p, partial, st);
+    const cudaError_t err = launch_group_stats<T, false>(g, p, workspace, st);
     if (err != cudaSuccess) return err;
     const dim3 grid((rows + g.row_block - 1) / g.row_block, g.slabs);
     return with_units(g.units, [&](auto u) {
@@ -2773,8 +2784,22 @@ extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, 
   const cudaError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
     const GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
+    unsigned char* base = static_cast<unsigned char*>(workspace);
+    if (g.parts > 0) {
+      float* values = reinterpret_cast<float*>(base);
+      const GroupNormExtra extra{reinterpret_cast<GroupStat*>(base + g.stat), reinterpret_cast<float*>(base + g.top_b)};
+      const cudaError_t err = g.units == kWhole ? launch_group_norm_one<T, kWhole, true>(g, p, values, extra, st)
+                                                : launch_group_norm_one<T, kStraddle, true>(g, p, values, extra, st);
+      if (err != cudaSuccess) return err;
+      const int teams = channels <= 1024 ? kRowThreads / 32 : 1;
+      const dim3 grid(std::min((rows + teams - 1) / teams, 8 * ds->sms));
+      auto kernel = channels <= 1024   ? group_rows_kernel<T, 8, 1>
+                    : channels <= 8192 ? group_rows_kernel<T, 8, 8>
+                                       : group_rows_kernel<T, 0, 8>;
+      return launch_pdl(kernel, grid, dim3(kRowThreads), 0, st, p, static_cast<const float*>(values), extra, q, scale);
+    }
     GroupSum* partial = static_cast<GroupSum*>(workspace);
-    cudaError_t err = launch_group_stats<T, true>(g, p, partial, st);
+    cudaError_t err = launch_group_stats<T, true>(g, p, workspace, st);
     if (err != cudaSuccess) return err;
     const dim3 grid((rows + g.row_block - 1) / g.row_block);
     const size_t smem = (sizeof(GroupStat) + sizeof(float4)) * groups;
@@ -2786,7 +2811,9 @@ extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, 
     static bool attr_set[4][kMaxDevices];
     const int which = !vec ? 0 : channels <= 1024 ? 1 : channels <= 8192 ? 2 : 3;
     if ((err = allow_smem(kernel, 4096 * 32, attr_set[which])) != cudaSuccess) return err;
-    return launch_pdl(kernel, grid, dim3(kRowThreads), smem, st, p, static_cast<const GroupSum*>(partial), q, scale);
+    const float* top_b = reinterpret_cast<const float*>(static_cast<unsigned char*>(workspace) + g.top_b);
+    return launch_pdl(kernel, grid, dim3(kRowThreads), smem, st, p, static_cast<const GroupSum*>(partial), top_b, q,
+                      scale);
   });
   if (e != cudaSuccess) return to_code(e);
   return to_code(cudaGetLastError());

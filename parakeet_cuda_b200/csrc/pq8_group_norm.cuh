@@ -11,7 +11,7 @@
 // quantised every value goes to fp64 at once: integers next to a border need
 // the statistics to more digits.
 //
-// Two forms. Where a window's rows of a few groups fit the shared memory of a
+// Two forms of each. Where a window's rows of a few groups fit the shared memory of a
 // cluster, one launch reads x once: every CTA holds its rows there, the
 // cluster's CTAs exchange their sums, and each normalises what it holds.
 // Otherwise (long windows of wide groups, rows that 16-byte loads do not fit)
@@ -254,10 +254,21 @@ __device__ __forceinline__ void load_unit(const T* p, float (&v)[kUnit<T, UNITS>
   if constexpr (UNITS == kScalar) v[0] = to_f32(p[0]);
   else load_chunk<T, kChunk<T>>(p, true, v);
 }
-template <typename T, int UNITS>
-__device__ __forceinline__ void store_unit(T* p, const float (&v)[kUnit<T, UNITS>]) {
-  if constexpr (UNITS == kScalar) p[0] = from_f32<T>(v[0]);
-  else store_chunk<T, kChunk<T>>(p, true, v);
+// E values of a unit, rounded to T once.
+template <typename T, int E>
+__device__ __forceinline__ void store_values(T* p, const float (&v)[E]) {
+  constexpr int C = kChunk<T>;
+  if constexpr (E == 1) {
+    p[0] = from_f32<T>(v[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i += C) {
+      float u[C];
+#pragma unroll
+      for (int j = 0; j < C; ++j) u[j] = v[i + j];
+      store_chunk<T, C>(p + i, true, u);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -272,9 +283,18 @@ __device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
   return v;
 }
 
-template <typename T, int UNITS>
+// QUANT: the first half of the quantised form. Its rows need every channel for
+// their scale, which no CTA here has: the values go to a workspace in fp32, with
+// the statistics for the ones next to a border (group_rows_kernel).
+struct GroupNormExtra {
+  GroupStat* stat;  // [windows][groups]
+  float* top_b;     // max|b|
+};
+template <typename T, int UNITS, bool QUANT>
 __global__ void __launch_bounds__(kNormThreads)
-    group_norm_kernel(const GroupNormParams p, T* __restrict__ y) {
+    group_norm_kernel(const GroupNormParams p, std::conditional_t<QUANT, float, T>* __restrict__ y,
+                      const GroupNormExtra extra) {
+  using Out = std::conditional_t<QUANT, float, T>;
   constexpr int E = kUnit<T, UNITS>;
   extern __shared__ uint4 held[];  // [rows][units]; then the slab's sums and statistics
   __shared__ GroupSum2 red[kNormThreads];
@@ -308,7 +328,7 @@ __global__ void __launch_bounds__(kNormThreads)
   GroupSum2 acc{{0.0, 0.0}, {0.0, 0.0}};
   int g, split;
   unit_group<UNITS, E>(min(sh.x, sh.units - 1), cg, &g, &split);  // the same for all of a thread's units
-  UnitSum<UNITS, E, false> sum(split, first_value<T>(p, lo, hi, g0, g, cg),
+  UnitSum<UNITS, E, QUANT> sum(split, first_value<T>(p, lo, hi, g0, g, cg),
                                UNITS == kStraddle && split < E ? first_value<T>(p, lo, hi, g0, g + 1, cg) : 0.0);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -351,6 +371,12 @@ __global__ void __launch_bounds__(kNormThreads)
       t = sums[g];
     }
     stat[g] = group_stat(t, first_value<T>(p, lo, hi, g0, g, cg), static_cast<double>(max(hi - lo, 1)) * cg, p.eps);
+    if (QUANT && part == 0) extra.stat[static_cast<size_t>(blockIdx.y) * p.groups + g0 + g] = stat[g];
+  }
+  if (QUANT && part == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
+    __shared__ float warp_top[kNormThreads / 32];
+    const float top = cta_max_abs(p.b, p.channels, warp_top);
+    if (threadIdx.x == 0) *extra.top_b = top;
   }
   __syncthreads();
   if (parts > 1) cluster_arrive_relaxed();  // this CTA has read the others' sums
@@ -358,18 +384,18 @@ __global__ void __launch_bounds__(kNormThreads)
     for (int u = sh.x; u < sh.units; u += sh.tx) {
       const int col = g0 * cg + u * E;
       const UnitNorm<UNITS, E> norm(p, stat, u, cg, ng, col);
-      T* const yu = y + col;
+      Out* const yu = y + col;
       float v[E];
 #pragma unroll 2
       for (int r = r0 + sh.y; r < held_end; r += sh.ty) {
         load_unit<T, UNITS>(reinterpret_cast<const T*>(held + static_cast<size_t>(r - r0) * sh.units + u), v);
         norm.apply(v, p.epi, p.round_out);
-        store_unit<T, UNITS>(yu + static_cast<size_t>(r) * p.channels, v);
+        store_values(yu + static_cast<size_t>(r) * p.channels, v);
       }
       for (int r = held_end + sh.y; r < r1; r += sh.ty) {
         load_unit<T, UNITS>(x + static_cast<size_t>(r) * p.channels + u * E, v);
         norm.apply(v, p.epi, p.round_out);
-        store_unit<T, UNITS>(yu + static_cast<size_t>(r) * p.channels, v);
+        store_values(yu + static_cast<size_t>(r) * p.channels, v);
       }
     }
   }
@@ -413,11 +439,16 @@ __device__ __forceinline__ void block_windows(const GroupNormParams& p, int b0, 
 // Sums of one block of rows for the groups of one slab.
 template <typename T, int UNITS, bool EXACT>
 __global__ void __launch_bounds__(kNormThreads)
-    group_stats_kernel(const GroupNormParams p, GroupSum* __restrict__ partial) {
+    group_stats_kernel(const GroupNormParams p, GroupSum* __restrict__ partial, float* __restrict__ top_b) {
   constexpr int E = kUnit<T, UNITS>;
   __shared__ GroupSum2 red[kNormThreads];
   griddep_wait();
   griddep_launch();
+  if (EXACT && blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) {  // max|b|, for the quantisation's error bound
+    __shared__ float warp_top[kNormThreads / 32];
+    const float top = cta_max_abs(p.b, p.channels, warp_top);
+    if (threadIdx.x == 0) *top_b = top;
+  }
   const int cg = p.channels / p.groups, g0 = static_cast<int>(blockIdx.y) * p.slab, ng = min(p.slab, p.groups - g0);
   const SlabShape<E> sh(ng * cg);
   const T* const x = static_cast<const T*>(p.x) + static_cast<size_t>(g0) * cg;
@@ -522,14 +553,14 @@ __global__ void __launch_bounds__(kNormThreads)
 #pragma unroll
           for (int k = 0; k < kAhead; ++k) {
             norm.apply(v[k], p.epi, p.round_out);
-            store_unit<T, UNITS>(yu + static_cast<size_t>(r + k * sh.ty) * p.channels, v[k]);
+            store_values(yu + static_cast<size_t>(r + k * sh.ty) * p.channels, v[k]);
           }
         }
         for (; r < r1; r += sh.ty) {
           float v[E];
           load_unit<T, UNITS>(xu + static_cast<size_t>(r) * p.channels, v);
           norm.apply(v, p.epi, p.round_out);
-          store_unit<T, UNITS>(yu + static_cast<size_t>(r) * p.channels, v);
+          store_values(yu + static_cast<size_t>(r) * p.channels, v);
         }
       }
     }
@@ -540,12 +571,11 @@ __global__ void __launch_bounds__(kNormThreads)
 // scale needs every channel.
 template <typename T, int CHUNKS, int WARPS, bool VEC>
 __global__ void __launch_bounds__(kRowThreads, 2)
-    group_quantize_kernel(const GroupNormParams p, const GroupSum* __restrict__ partial, int8_t* __restrict__ q,
-                          float* __restrict__ scale) {
+    group_quantize_kernel(const GroupNormParams p, const GroupSum* __restrict__ partial,
+                          const float* __restrict__ top_b, int8_t* __restrict__ q, float* __restrict__ scale) {
   extern __shared__ GroupStat stat[];  // [groups], then their fp32 form
   float4* const fast = reinterpret_cast<float4*>(stat + p.groups);
   __shared__ double team_smem[2 * WARPS];
-  __shared__ float warp_top[kRowThreads / 32];
   constexpr int kTeams = kRowThreads / (32 * WARPS);
   const RowTeam<WARPS> team{team_smem};
   griddep_wait();
@@ -559,9 +589,16 @@ __global__ void __launch_bounds__(kRowThreads, 2)
   src.whole = src.group_width % kChunk<T> == 0;
   src.inv_width = 1.0f / src.group_width;
   src.epi = p.epi;
-  src.top_b = cta_max_abs(p.b, p.channels, warp_top);
+  src.top_b = __ldg(top_b);
   const int b0 = static_cast<int>(blockIdx.x) * p.row_block;
   const int b1 = static_cast<int>(min(static_cast<long long>(b0) + p.row_block, static_cast<long long>(p.rows)));
+  if constexpr (WARPS == 1) {  // this warp's first row on its way to L1 while the statistics are put together
+    const int r = b0 + (static_cast<int>(threadIdx.x) >> 5);
+    const T* const x = static_cast<const T*>(p.x) + static_cast<size_t>(r) * p.channels;
+    if (r < b1)
+      for (int c = (threadIdx.x & 31) * 128 / static_cast<int>(sizeof(T)); c < p.channels; c += 32 * 128 / static_cast<int>(sizeof(T)))
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(x + c));
+  }
   block_windows(p, b0, b1, [&](int w, int lo, int hi, int r0, int r1) {
     group_finish<T>(p, partial, w, lo, hi, 0, p.groups, stat);
     for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
@@ -576,6 +613,72 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       if (team.index() == 0) scale[r] = s;
     }
   });
+}
+
+// The second half of the quantised form where the first was one launch: rows of
+// normalised fp32 values (error within error()) to integers; exact values
+// from x and the statistics.
+template <typename T>
+struct NormedSource {
+  static constexpr bool kExact = false, kLayerNorm = false;
+  static constexpr int E = 4;
+  const float* y;
+  const T* x;
+  const float* w;
+  const float* b;
+  const GroupStat* stat;  // of the row's window
+  float inv_width;        // groups / channels
+  int epi;
+  float top_b;
+  __device__ __forceinline__ void raw(int c, float (&v)[E]) const { load_chunk<float, E>(y + c * E, true, v); }
+  __device__ __forceinline__ void value(int, float (&)[E]) const {}
+  __device__ __forceinline__ double exact(int col) const {
+    const GroupStat s = stat[static_cast<int>((static_cast<float>(col) + 0.5f) * inv_width)];
+    const double z = (static_cast<double>(to_f32(x[col])) - s.mean) * s.rstd * static_cast<double>(w[col]) +
+                     static_cast<double>(b[col]);
+    return act_f64(z, epi);
+  }
+  __device__ __forceinline__ float error(float h) const { return 0x1p-20f * (h + top_b + 1.0f); }
+};
+
+// Window of row r, or -1.
+__device__ __forceinline__ int row_window(const GroupNormParams& p, int r) {
+  if (p.offsets == nullptr) return r / (p.rows / p.windows);
+  int a = 0, b = p.windows;  // the first window that ends after r is in [a, b]
+  while (a < b) {
+    const int mid = (a + b) >> 1;
+    if (__ldg(p.offsets + mid + 1) <= r) a = mid + 1;
+    else b = mid;
+  }
+  return a < p.windows && __ldg(p.offsets + a) <= r ? a : -1;
+}
+
+template <typename T, int CHUNKS, int WARPS>
+__global__ void __launch_bounds__(kRowThreads, 3)
+    group_rows_kernel(const GroupNormParams p, const float* __restrict__ y, const GroupNormExtra extra,
+                      int8_t* __restrict__ q, float* __restrict__ scale) {
+  __shared__ double team_smem[2 * WARPS];
+  constexpr int kTeams = kRowThreads / (32 * WARPS);
+  const RowTeam<WARPS> team{team_smem};
+  griddep_wait();
+  griddep_launch();
+  NormedSource<T> src;
+  src.w = p.w;
+  src.b = p.b;
+  src.inv_width = 1.0f / static_cast<float>(p.channels / p.groups);
+  src.epi = p.epi;
+  src.top_b = __ldg(extra.top_b);
+  const int first = static_cast<int>(blockIdx.x) * kTeams + static_cast<int>(threadIdx.x) / (32 * WARPS);
+  for (int row = first; row < p.rows; row += static_cast<int>(gridDim.x) * kTeams) {
+    const int w = row_window(p, row);
+    if (w < 0) continue;  // the whole team
+    const size_t at = static_cast<size_t>(row) * p.channels;
+    src.y = y + at;
+    src.x = static_cast<const T*>(p.x) + at;
+    src.stat = extra.stat + static_cast<size_t>(w) * p.groups;
+    const float s = quantize_row<CHUNKS, WARPS>(src, p.channels, q + at, team);
+    if (team.index() == 0) scale[row] = s;
+  }
 }
 
 }  // namespace pq8
