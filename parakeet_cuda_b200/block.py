@@ -25,6 +25,12 @@ The reference launches the same block per window as one SGEMM plus an
 elementwise kernel per linear after a ``dequant_q8`` of the layer's weights
 (``parakeet_cuda/encoder.py:28-127``); here the Q8_0 weights stay resident and
 packed, the epilogues are fused, and all windows share every launch.
+
+``EncoderBlocks(products='int8')`` runs the linears as products of 8-bit integers
+instead (``Runtime.linear_i8``): the Q8_0 weights are requantised with one scale per
+output channel when the blocks are made, tokens are quantised per row on the way
+into each linear - with the LayerNorm in front of it in the same pass - and the FFN hidden state is
+bfloat16. Everything else (attention, depthwise convolution, residual stream) is as above.
 """
 from __future__ import annotations
 
@@ -42,13 +48,21 @@ class EncoderBlocks:
     """``layers`` encoder blocks over ``windows`` windows of ``t`` frames on one device."""
 
     def __init__(self, model, runtime: Runtime, windows: int, t: int, layers: int = 24,
-                 attention_fp32: bool = False, sequences: bool = True):
+                 attention_fp32: bool = False, sequences: bool = True, products: str = 'tf32'):
+        if products not in ('tf32', 'int8'):
+            raise ValueError(f"products must be 'tf32' or 'int8', got {products!r}")
+        self.int8 = products == 'int8'
+        sequences = sequences and not self.int8
         self.rt, self.windows, self.t, self.layers = runtime, windows, t, layers
         self.rows = windows * t
         self.attn_flags = FLAG_OUT_TF32 | (ATTN_FP32 if attention_fp32 else 0)
         dev = runtime.device
-        # packed Q8_0 linears (device repack), the same set as the linear stack
-        self.linears = EncoderStack(model, runtime, 1, layers=layers).weights
+        if self.int8:  # requantised with a scale per output channel
+            self.linears = [{name: runtime.int8_weight((np.concatenate(
+                [np.asarray(model.raw(f'encoder.layers.{l}.{key}.weight'), np.uint8).reshape(-1) for key in keys]), n, k))
+                for name, keys, n, k, *_ in LAYER_PLAN} for l in range(layers)]
+        else:  # packed Q8_0 linears (device repack), the same set as the linear stack
+            self.linears = EncoderStack(model, runtime, 1, layers=layers).weights
         f32 = dict(dtype=torch.float32, device=dev)
         to_dev = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.float32)).to(dev)
         self.params = []
@@ -74,7 +88,7 @@ class EncoderBlocks:
         self.buf = {
             'x': torch.zeros(rows, D_MODEL, **f32),
             'norm': torch.empty(rows, D_MODEL, **f32),
-            'hidden': torch.empty(rows, D_FF, **f32),
+            'hidden': torch.empty(rows, D_FF, dtype=torch.bfloat16 if self.int8 else torch.float32, device=dev),
             'qkv': torch.empty(rows, 3 * D_MODEL, **f32),
             'pos': torch.empty(2 * t - 1, D_MODEL, **f32),
             'ctx': torch.empty(rows, D_MODEL, **f32),
@@ -133,11 +147,50 @@ class EncoderBlocks:
         self.rt.gemm(x, self.linears[l][name], out=out, resid=resid, epilogue=epi, alpha=alpha,
                      flags=flags | FLAG_X_TF32)
 
+    def _linear_i8(self, l: int, name: str, src, dst: str, norm: str | None = None) -> None:
+        """The linear in 8-bit integers on the block's buffers, after the LayerNorm ``norm``."""
+        epi, alpha = self._plan[name][4:6]
+        x = self.buf[src] if isinstance(src, str) else src
+        out = self.buf[dst]
+        self.rt.linear_i8(x, self.linears[l][name], out=out, resid=out if epi == EPI_RESIDUAL else None, epilogue=epi,
+                          alpha=alpha, norm=None if norm is None else self.params[l][norm])
+
+    def _layer_int8(self, l: int, final_norm: bool) -> None:
+        """``layer`` with the products in 8-bit integers."""
+        p = self.params[l]
+        self._linear_i8(l, 'ffn1_up', 'x', 'hidden', 'norm_feed_forward1')
+        self._linear_i8(l, 'ffn1_down', 'hidden', 'x')
+        self._linear_i8(l, 'qkv', 'x', 'qkv', 'norm_self_att')
+        self._linear_i8(l, 'pos', self.pe, 'pos')
+        self._attention(p)
+        self._linear_i8(l, 'out', 'ctx', 'x')
+        self._linear_i8(l, 'pw1_glu', 'x', 'gate', 'norm_conv')
+        self._depthwise(p)
+        self._linear_i8(l, 'pw2', 'dw', 'x')
+        self._linear_i8(l, 'ffn2_up', 'x', 'hidden', 'norm_feed_forward2')
+        self._linear_i8(l, 'ffn2_down', 'hidden', 'x')
+        if final_norm:
+            self._ln(l, 'norm_out', 'x', 'x', tf32=False)
+
+    def _attention(self, p) -> None:
+        b = self.buf
+        self.rt.lib.call('pq8_rel_attention', b['qkv'].data_ptr(), b['pos'].data_ptr(), p['u'].data_ptr(),
+                         p['v'].data_ptr(), b['ctx'].data_ptr(), self.windows, self.t, self.attn_flags,
+                         self.attn_ws.data_ptr(), self.attn_ws.numel(), self.rt.stream())
+
+    def _depthwise(self, p) -> None:
+        b, (bw, bb, bm, bv) = self.buf, p['bn']
+        self.rt.lib.call('pq8_conv_depthwise_bn_silu', b['gate'].data_ptr(), p['dw'].data_ptr(), bw.data_ptr(),
+                         bb.data_ptr(), bm.data_ptr(), bv.data_ptr(), b['dw'].data_ptr(), self.windows, self.t, D_MODEL,
+                         FLAG_OUT_TF32, self.rt.stream())
+
     def layer(self, l: int, final_norm: bool = True) -> None:
         """One block on the residual stream ``buf['x']`` (reference.py:33-66).
         ``final_norm=False`` leaves out the block's last LayerNorm (``norm_out``)
         and keeps the residual stream as it stands before it."""
-        b, p, lib, st = self.buf, self.params[l], self.rt.lib, self.rt.stream()
+        if self.int8:
+            return self._layer_int8(l, final_norm)
+        p = self.params[l]
         seq = self.seq_plans is not None
         self._ln(l, 'norm_feed_forward1', 'x', 'norm')
         if seq:
@@ -151,16 +204,11 @@ class EncoderBlocks:
         else:
             self._gemm(l, 'qkv', 'norm', 'qkv')
             self._gemm(l, 'pos', self.pe, 'pos')
-        lib.call('pq8_rel_attention', b['qkv'].data_ptr(), b['pos'].data_ptr(), p['u'].data_ptr(), p['v'].data_ptr(),
-                 b['ctx'].data_ptr(), self.windows, self.t, self.attn_flags, self.attn_ws.data_ptr(),
-                 self.attn_ws.numel(), st)
+        self._attention(p)
         self._gemm(l, 'out', 'ctx', 'x')
         self._ln(l, 'norm_conv', 'x', 'norm')
         self._gemm(l, 'pw1_glu', 'norm', 'gate', out_tf32=False)  # the depthwise conv reads it, not a GEMM
-        bw, bb, bm, bv = p['bn']
-        lib.call('pq8_conv_depthwise_bn_silu', b['gate'].data_ptr(), p['dw'].data_ptr(), bw.data_ptr(),
-                 bb.data_ptr(), bm.data_ptr(), bv.data_ptr(), b['dw'].data_ptr(), self.windows, self.t, D_MODEL,
-                 FLAG_OUT_TF32, st)
+        self._depthwise(p)
         self._gemm(l, 'pw2', 'dw', 'x')
         self._ln(l, 'norm_feed_forward2', 'x', 'norm')
         if seq:
