@@ -2152,30 +2152,36 @@ int check_rows_args(const void* x, int type, long long ld, const float* w, const
   return PQ8_OK;
 }
 
-template <typename T, int CHUNKS, int WARPS, bool VEC>
+template <typename T, int CHUNKS, int WARPS, bool FULL, bool VEC>
 cudaError_t launch_rows(DeviceState* ds, const T* x, long long ld, const float* w, const float* b, int8_t* q,
                         float* scale, int rows, int width, cudaStream_t st) {
   constexpr int kTeams = kRowThreads / (32 * WARPS);
   const dim3 grid(static_cast<unsigned>(std::min<long long>((rows + kTeams - 1LL) / kTeams, 8LL * ds->sms)));
   if (w != nullptr)
-    return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, true, VEC>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
+    return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, FULL, true, VEC>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
                       kNormEps64, q, scale, rows, width);
-  return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, false, VEC>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
+  return launch_pdl(quantize_rows_kernel<T, CHUNKS, WARPS, FULL, false, VEC>, grid, dim3(kRowThreads), 0, st, x, ld, w, b,
                     kNormEps64, q, scale, rows, width);
 }
 
 // A warp per row while 32 lanes x 32 values hold it, then a CTA per row while
 // 256 x 32 do; rows read again in each pass past that and where 16-byte loads
-// do not fit.
+// do not fit. The widths that fill a thread's chunks exactly, or half of
+// them, have kernels without checks for missing ones (24,000 rows of 1024 bf16:
+// XX us against YY).
 template <typename T>
 cudaError_t launch_rows_typed(DeviceState* ds, const T* x, long long ld, const float* w, const float* b, int8_t* q,
                               float* scale, int rows, int width, cudaStream_t st) {
   constexpr int C = 32 / kChunk<T>;
   const bool vec = aligned(x, 16) && (rows == 1 || (ld * sizeof(T)) % 16 == 0) && aligned(w, 16) && aligned(b, 16);
-  if (!vec) return launch_rows<T, 0, 8, false>(ds, x, ld, w, b, q, scale, rows, width, st);
-  if (width <= 1024) return launch_rows<T, C, 1, true>(ds, x, ld, w, b, q, scale, rows, width, st);
-  if (width <= 8192) return launch_rows<T, C, 8, true>(ds, x, ld, w, b, q, scale, rows, width, st);
-  return launch_rows<T, 0, 8, true>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (!vec) return launch_rows<T, 0, 8, false, false>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (width == 512) return launch_rows<T, C / 2, 1, true, true>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (width == 1024) return launch_rows<T, C, 1, true, true>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (width <= 1024) return launch_rows<T, C, 1, false, true>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (width == 4096) return launch_rows<T, C / 2, 8, true, true>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (width == 8192) return launch_rows<T, C, 8, true, true>(ds, x, ld, w, b, q, scale, rows, width, st);
+  if (width <= 8192) return launch_rows<T, C, 8, false, true>(ds, x, ld, w, b, q, scale, rows, width, st);
+  return launch_rows<T, 0, 8, false, true>(ds, x, ld, w, b, q, scale, rows, width, st);
 }
 
 int quantize_rows(const void* x, int type, long long ld, const float* w, const float* b, int8_t* q, float* scale,
@@ -2793,9 +2799,10 @@ extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, 
       if (err != cudaSuccess) return err;
       const int teams = channels <= 1024 ? kRowThreads / 32 : 1;
       const dim3 grid(std::min((rows + teams - 1) / teams, 8 * ds->sms));
-      auto kernel = channels <= 1024   ? group_rows_kernel<T, 8, 1>
-                    : channels <= 8192 ? group_rows_kernel<T, 8, 8>
-                                       : group_rows_kernel<T, 0, 8>;
+      auto kernel = channels == 1024   ? group_rows_kernel<T, 8, 1, true>
+                    : channels <= 1024 ? group_rows_kernel<T, 8, 1, false>
+                    : channels <= 8192 ? group_rows_kernel<T, 8, 8, false>
+                                       : group_rows_kernel<T, 0, 8, false>;
       return launch_pdl(kernel, grid, dim3(kRowThreads), 0, st, p, static_cast<const float*>(values), extra, q, scale);
     }
     GroupSum* partial = static_cast<GroupSum*>(workspace);

@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     __syncthreads();
     for (int r = r0 + static_cast<int>(threadIdx.x) / (32 * WARPS); r < r1; r += kTeams) {
       src.x = static_cast<const T*>(p.x) + static_cast<size_t>(r) * p.channels;
-      const float s = quantize_row<CHUNKS, WARPS>(src, p.channels, q + static_cast<size_t>(r) * p.channels, team);
+      const float s = quantize_row<CHUNKS, WARPS, false>(src, p.channels, q + static_cast<size_t>(r) * p.channels, team);
       if (team.index() == 0) scale[r] = s;
     }
   });
@@ -653,7 +653,7 @@ __device__ __forceinline__ int row_window(const GroupNormParams& p, int r) {
   return a < p.windows && __ldg(p.offsets + a) <= r ? a : -1;
 }
 
-template <typename T, int CHUNKS, int WARPS>
+template <typename T, int CHUNKS, int WARPS, bool FULL>
 __global__ void __launch_bounds__(kRowThreads, 3)
     group_rows_kernel(const GroupNormParams p, const float* __restrict__ y, const GroupNormExtra extra,
                       int8_t* __restrict__ q, float* __restrict__ scale) {
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
     src.y = y + at;
     src.x = static_cast<const T*>(p.x) + at;
     src.stat = extra.stat + static_cast<size_t>(w) * p.groups;
-    const float s = quantize_row<CHUNKS, WARPS>(src, p.channels, q + at, team);
+    const float s = quantize_row<CHUNKS, WARPS, FULL>(src, p.channels, q + at, team);
     if (team.index() == 0) scale[row] = s;
   }
 }

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kI8GemvThreads, 2) i8_gemv_kernel(const I8Para
     const int r = kTeam > 1 ? 0 : threadIdx.x >> 5;
     if (r < p.m) {
       src.x = static_cast<const T*>(tokens.x) + r * tokens.ld;
-      const float s = quantize_row<32 / kChunk<T>, kTeam>(src, p.k, q + r * p.k, team);
+      const float s = quantize_row<32 / kChunk<T>, kTeam, false>(src, p.k, q + r * p.k, team);
       if (team.index() == 0) scale_smem[r] = s;
     }
     __syncthreads();

@@ -358,27 +358,30 @@ struct GroupNormSource {
 // ---------------------------------------------------------------------------
 // One row, by a team of WARPS warps. CHUNKS > 0: each thread holds up to CHUNKS
 // chunks of the row in registers (width <= CHUNKS * E * 32 * WARPS);
-// CHUNKS == 0: any width, read again in each pass. `width` is a multiple of
-// E; q is E-byte aligned. Every thread of the team returns the scale.
+// CHUNKS == 0: any width, read again in each pass. FULL: the width is exactly
+// that of CHUNKS chunks per thread, so that no chunk has to be checked for.
+// `width` is a multiple of E; q is E-byte aligned. Every thread of the team
+// returns the scale.
 //
 // Per value, the common path is a multiply-add that rounds (adding 1.5 x
 // 2^23 leaves the nearest integer in the low bits), its remainder, and a
 // running maximum of the remainders: a thread looks its values through for
 // the ones next to a border only when that maximum says there is one.
-template <int CHUNKS, int WARPS, typename Src>
+template <int CHUNKS, int WARPS, bool FULL, typename Src>
 __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, const RowTeam<WARPS>& team) {
   constexpr int E = Src::E;
   constexpr int kThreads = WARPS * 32;
   constexpr bool kCached = CHUNKS > 0;
   constexpr int N = kCached ? CHUNKS : 1;
-  const int tid = team.index(), chunks = width / E;
+  const int tid = team.index(), chunks = FULL ? CHUNKS * kThreads : width / E;
+  auto has = [&](int c) { return FULL || c < chunks; };
   static_assert(N * E <= 32, "a mask bit per value");
   float v[N][E];
   if constexpr (kCached) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = tid + j * kThreads;
-      if (c < chunks) src.raw(c, v[j]);
+      if (has(c)) src.raw(c, v[j]);
     }
   }
   // f(values, chunk) for every chunk of this thread; `compute`: from the raw
@@ -388,7 +391,7 @@ __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, con
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const int c = tid + j * kThreads;
-        if (c < chunks) {
+        if (has(c)) {
           if (compute) src.value(c, v[j]);
           f(v[j], c);
         }
@@ -414,7 +417,7 @@ __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, con
     if constexpr (kCached) {
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (tid + j * kThreads < chunks) found |= pick_chunk(v[j]) << (j * E);
+        if (has(tid + j * kThreads)) found |= pick_chunk(v[j]) << (j * E);
       for (; found; found &= found - 1) {
         const int bit = __ffs(found) - 1;
         f((tid + (bit / E) * kThreads) * E + bit % E);
@@ -434,7 +437,7 @@ __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, con
     if constexpr (kCached) {
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (tid + j * kThreads < chunks) src.add(v[j], first, s, sq);
+        if (has(tid + j * kThreads)) src.add(v[j], first, s, sq);
     } else {
       for (int c = tid; c < chunks; c += kThreads) {
         src.raw(c, v[0]);
@@ -445,12 +448,16 @@ __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, con
   }
 
   float mine = 0.0f, bad = 0.0f;
-  each([&](const float(&u)[E], int) {
+  float chunk_top[N];  // cached rows: the largest of each chunk
+  each([&](const float(&u)[E], int c) {
+    float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      mine = fmaxf(mine, fabsf(u[i]));
+      m = fmaxf(m, fabsf(u[i]));
       bad = fmaf(u[i], 0.0f, bad);  // NaN from an infinity or a NaN on
     }
+    mine = fmaxf(mine, m);
+    if constexpr (kCached) chunk_top[(c - tid) / kThreads] = m;
   }, true);
   const float top = team.max(bad == 0.0f ? mine : INFINITY);
   float s = top / 127.0f;
@@ -459,9 +466,22 @@ __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, con
       // the values that may be the largest, exactly
       const float least = top - 2.5f * src.error(top);
       double t64 = 0.0;
-      if (mine >= least)
-        columns([&](float u) { return fabsf(u) >= least; },
-                [&](int col) { t64 = fmax(t64, ::fabs(src.exact(col))); });
+      if (mine >= least) {
+        if constexpr (kCached) {
+          uint32_t found = 0;
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (has(tid + j * kThreads) && chunk_top[j] >= least) found |= 1u << j;
+          for (; found; found &= found - 1) {
+            const int col = (tid + (__ffs(found) - 1) * kThreads) * E;
+#pragma unroll 1
+            for (int i = 0; i < E; ++i) t64 = fmax(t64, ::fabs(src.exact(col + i)));
+          }
+        } else {
+          columns([&](float u) { return fabsf(u) >= least; },
+                  [&](int col) { t64 = fmax(t64, ::fabs(src.exact(col))); });
+        }
+      }
       s = static_cast<float>(team.max(t64) * (1.0 / 127.0));
     }
   }
@@ -519,7 +539,7 @@ constexpr int kRowThreads = 256;
 // warps up to 8192 (the row stays in registers in both), and past that, or
 // where 16-byte loads do not fit, the CTA reads the row again in each pass.
 // NORM: LayerNorm first.
-template <typename T, int CHUNKS, int WARPS, bool NORM, bool VEC>
+template <typename T, int CHUNKS, int WARPS, bool FULL, bool NORM, bool VEC>
 __global__ void __launch_bounds__(kRowThreads, NORM ? 3 : 4)
     quantize_rows_kernel(const T* __restrict__ x, long long ld, const float* __restrict__ w,
                          const float* __restrict__ b, double eps, int8_t* __restrict__ q, float* __restrict__ scale,
@@ -541,7 +561,7 @@ __global__ void __launch_bounds__(kRowThreads, NORM ? 3 : 4)
   const int first = static_cast<int>(blockIdx.x) * kTeams + static_cast<int>(threadIdx.x) / (32 * WARPS);
   for (long long row = first; row < rows; row += static_cast<long long>(gridDim.x) * kTeams) {
     src.x = x + row * ld;
-    const float s = quantize_row<CHUNKS, WARPS>(src, width, q + row * width, team);
+    const float s = quantize_row<CHUNKS, WARPS, FULL>(src, width, q + row * width, team);
     if (team.index() == 0) scale[row] = s;
   }
 }
