@@ -287,8 +287,12 @@ struct LayerNormSource {
     float g[E], h[E];
     load_params<E>(w + c * E, VEC, g);
     load_params<E>(b + c * E, VEC, h);
+    const f32x2 hi = pack2(-mean_hi, -mean_hi), lo = pack2(-mean_lo, -mean_lo), r2 = pack2(rs, rs);
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = fmaf(((v[i] - mean_hi) - mean_lo) * rs, g[i], h[i]);
+    for (int i = 0; i < E; i += 2) {
+      const f32x2 d = mul2(add2(add2(pack2(v[i], v[i + 1]), hi), lo), r2);
+      unpack2(fma2(d, pack2(g[i], g[i + 1]), pack2(h[i], h[i + 1])), &v[i], &v[i + 1]);
+    }
   }
   __device__ __forceinline__ double exact(int col) const {
     return (static_cast<double>(to_f32(x[col])) - mean) * rstd * static_cast<double>(w[col]) +
@@ -507,7 +511,7 @@ __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, con
     for (int i = 0; i < E; ++i) {
       const float big = fmaf(u[i], inv, kBig);
       m[i] = __float_as_uint(big);
-      worst = fmaxf(worst, fabsf(fmaf(u[i], inv, kBig - big)));
+      worst = fmaxf(worst, fabsf(fmaf(u[i], inv, kBig - big)));  // what the rounding took off
     }
 #pragma unroll
     for (int i = 0; i < E; i += 4)
