@@ -487,7 +487,8 @@ PQ8_API int pq8_stem(const float* mel, int windows, int frames, const float* w0,
  * q = 0; a row that holds an infinity or a NaN has s = NaN and q = 0, so that
  * its outputs are NaN and no other row's.
  * Types are PQ8_TYPE_*; ld is the distance of two rows in elements (>= width).
- * `width` / `k` is a positive multiple of 16, q 16-byte aligned and dense.
+ * `width` / `k` is a positive multiple of 16, q 16-byte aligned and dense; rows
+ * at most 2^30. Outputs, scales and workspaces overlap no input.
  * x needs its type's alignment only; rows whose start and distance are
  * multiples of 16 bytes are read fastest. */
 PQ8_API int pq8_quantize_rows(const void* x, int type, long long ld, int8_t* q, float* scale, int rows, int width,
@@ -505,7 +506,9 @@ PQ8_API int pq8_layer_norm_quantize(const void* x, int type, long long ld, const
  * PQ8_EPI_GLU takes plain rows (y[:, j] = z[:, j] sigmoid(z[:, j + n / 2]), n
  * even: no packed layout). bias: float[n] or NULL; resid: y's type and
  * shape (EPI_RESIDUAL only), may be y itself. y may overlap none of the other inputs.
- * k at most 131,056, so that no sum leaves 32 bits. Any m >= 0, n >= 1. */
+ * The last bits of a SiLU or GLU output may depend on the token next to it (two
+ * share a reciprocal); everything else of a row is its own.
+ * k at most 131,056, so that no sum leaves 32 bits; m and n at most 2^30. */
 PQ8_API int pq8_gemm_i8(const int8_t* w, const float* w_scale, const int8_t* x, const float* x_scale, void* y,
                         int y_type, const float* bias, const void* resid, int m, int n, int k, int epilogue,
                         float alpha, void* stream);
@@ -534,7 +537,9 @@ PQ8_API int pq8_linear_i8(const int8_t* w, const float* w_scale, const void* x, 
  * concerned would get no defined values, though nothing outside y is touched),
  * rows of y in no window are not written; or NULL: windows of rows / windows rows each.
  * Sums are added in a fixed order, per column over at most 32 rows in FP32 (FP64
- * for the quantised form), FP64 above. channels at most 16384, groups at most
+ * for the quantised form), FP64 above; a group that holds an infinity or a NaN in a
+ * window becomes NaN there, and one with values over 2^60 apart may. eps from 1e-30
+ * to 1e30. channels at most 16384, groups at most
  * 4096, rows at most 2^30. y must not overlap x. PQ8_FLAG_OUT_TF32 (type F32)
  * rounds y for a following pq8_gemm. The workspace (16-byte aligned, no
  * initialisation) is per call in flight; where its size is 0 it may be NULL.

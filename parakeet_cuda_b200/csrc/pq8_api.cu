@@ -2091,6 +2091,7 @@ namespace {
 
 constexpr double kNormEps64 = 1e-5;  // reference.py:8
 constexpr int kI8MaxK = 131056;      // 128 * 128 * k stays below 2^31
+constexpr int kI8MaxRows = 1 << 30;  // tokens or channels: a tile past the last one still has a 32-bit index
 
 int type_size(int type) { return type == PQ8_TYPE_F32 ? 4 : type == PQ8_TYPE_F16 || type == PQ8_TYPE_BF16 ? 2 : 0; }
 
@@ -2129,7 +2130,7 @@ size_t rows_bytes(long long rows, long long ld, int width, int size) {
 }
 
 int check_token_args(const void* x, int type, long long ld, const float* w, const float* b, int rows, int width) {
-  if (rows < 0 || width <= 0 || width % 16 || width > kI8MaxK) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  if (rows < 0 || rows > kI8MaxRows || width <= 0 || width % 16 || width > kI8MaxK) return PQ8_ERR_UNSUPPORTED_SHAPE;
   const int size = type_size(type);
   if (size == 0 || (w == nullptr) != (b == nullptr)) return PQ8_ERR_INVALID_ARGUMENT;
   if (rows == 0) return PQ8_OK;
@@ -2146,10 +2147,12 @@ int check_rows_args(const void* x, int type, long long ld, const float* w, const
   if (q == nullptr || scale == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
   if (!aligned(q, 16) || !aligned(scale, 4)) return PQ8_ERR_MISALIGNED;
   const int size = type_size(type);
-  const size_t nx = rows_bytes(rows, ld, width, size);
-  if (overlap(x, nx, q, static_cast<size_t>(rows) * width) || overlap(x, nx, scale, static_cast<size_t>(rows) * 4))
-    return PQ8_ERR_INVALID_ARGUMENT;
-  return PQ8_OK;
+  const size_t nx = rows_bytes(rows, ld, width, size), nq = static_cast<size_t>(rows) * width,
+               ns = static_cast<size_t>(rows) * 4, nw = static_cast<size_t>(width) * 4;
+  const bool clash = overlap(q, nq, scale, ns) || overlap(x, nx, q, nq) || overlap(x, nx, scale, ns) ||
+                     overlap(w, nw, q, nq) || overlap(w, nw, scale, ns) || overlap(b, nw, q, nq) ||
+                     overlap(b, nw, scale, ns);
+  return clash ? PQ8_ERR_INVALID_ARGUMENT : PQ8_OK;
 }
 
 template <typename T, int CHUNKS, int WARPS, bool FULL, bool VEC>
@@ -2201,7 +2204,8 @@ int quantize_rows(const void* x, int type, long long ld, const float* w, const f
 
 int check_i8_args(const int8_t* w, const float* w_scale, const void* y, int y_type, const void* resid, int m, int n,
                   int k, int epilogue) {
-  if (m < 0 || n < 1 || k <= 0 || k % 16 || k > kI8MaxK) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  if (m < 0 || m > kI8MaxRows || n < 1 || n > kI8MaxRows || k <= 0 || k % 16 || k > kI8MaxK)
+    return PQ8_ERR_UNSUPPORTED_SHAPE;
   if (epilogue < PQ8_EPI_NONE || epilogue > PQ8_EPI_RESIDUAL || type_size(y_type) == 0)
     return PQ8_ERR_INVALID_ARGUMENT;
   if (epilogue == PQ8_EPI_GLU && n % 2) return PQ8_ERR_UNSUPPORTED_SHAPE;
@@ -2319,14 +2323,15 @@ int launch_i8_gemm(DeviceState* ds, const I8Params& p, int splits, cudaStream_t 
 // 640 to 16,384: e.g. 375 x 1024 x 1024 (tokens x K x channels) takes 5.1 us in
 // tiles of 32, 6.0 of 128, 7.3 of 256; 375 x 4096 x 1024 11.5 in tiles of 32 and
 // 9.9 of 128 with K in 4 splits; 3000 x 4096 x 1024 24 of 128, 17.4 of 192, 19.3
-// of 256; 12,000 x 1024 x 1024 49 of 32, 23 of 128, 19.6 of 192, 18.2 of 256.
+// of 256; 3000 x 1024 x 1024 10.9 of 192, 12.5 of 256; 12,000 x 1024 x 1024 49 of
+// 32, 23 of 128, 19.6 of 192, 18.2 of 256.
 struct I8Shape {
   int tokens, ctas;
   double fixed, per_block, per_tile, split;
 };
 constexpr I8Shape kI8Shapes[] = {{16, 1, 3.0, 0.255, 0.1, 1.1},  {32, 1, 3.0, 0.255, 0.15, 1.4},
                                  {64, 1, 3.2, 0.255, 0.45, 1.9}, {128, 1, 3.9, 0.26, 1.1, 2.5},
-                                 {192, 2, 4.4, 0.27, 1.6, 0.0},  {256, 2, 3.4, 0.31, 2.2, 0.0}};
+                                 {192, 2, 4.4, 0.27, 1.6, 0.0},  {256, 2, 3.9, 0.31, 2.2, 0.0}};
 
 struct I8Choice {
   int shape, splits;
@@ -2497,7 +2502,7 @@ extern "C" int pq8_gemm_i8(const int8_t* w, const float* w_scale, const int8_t* 
 
 extern "C" int pq8_linear_i8_workspace_size(int m, int k, size_t* bytes) {
   if (bytes == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
-  if (m < 0 || k <= 0 || k % 16 || k > kI8MaxK) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  if (m < 0 || m > kI8MaxRows || k <= 0 || k % 16 || k > kI8MaxK) return PQ8_ERR_UNSUPPORTED_SHAPE;
   *bytes = plan_linear_i8(m, k).total;
   return PQ8_OK;
 }
@@ -2515,12 +2520,21 @@ extern "C" int pq8_linear_i8(const int8_t* w, const float* w_scale, const void* 
   if (!fused && (workspace == nullptr || workspace_bytes < ws.total)) return PQ8_ERR_WORKSPACE;
   int8_t* q = fused ? nullptr : static_cast<int8_t*>(workspace);
   float* scale = fused ? nullptr : reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + ws.scale);
-  const size_t x_bytes = rows_bytes(m, ld, k, type_size(x_type));
-  if (!fused && overlap(x, x_bytes, workspace, ws.total)) return PQ8_ERR_INVALID_ARGUMENT;
+  const size_t x_bytes = rows_bytes(m, ld, k, type_size(x_type)), norm_bytes = static_cast<size_t>(k) * 4,
+               y_bytes = static_cast<size_t>(m) * (epilogue == PQ8_EPI_GLU ? n / 2 : n) * type_size(y_type);
   if ((rc = check_i8_overlap(w, w_scale, x, x_bytes, nullptr, y, y_type, bias, resid, m, n, k, epilogue))) return rc;
-  if (!fused && overlap(y, static_cast<size_t>(m) * (epilogue == PQ8_EPI_GLU ? n / 2 : n) * type_size(y_type),
-                        workspace, ws.total))
+  if (overlap(y, y_bytes, norm_w, norm_bytes) || overlap(y, y_bytes, norm_b, norm_bytes))
     return PQ8_ERR_INVALID_ARGUMENT;
+  if (!fused) {  // the workspace is written before everything but x and the norm is read
+    const struct {
+      const void* at;
+      size_t bytes;
+    } used[] = {{x, x_bytes}, {y, y_bytes}, {w, static_cast<size_t>(n) * k}, {w_scale, static_cast<size_t>(n) * 4},
+                {bias, static_cast<size_t>(n) * 4}, {epilogue == PQ8_EPI_RESIDUAL ? resid : nullptr, y_bytes},
+                {norm_w, norm_bytes}, {norm_b, norm_bytes}};
+    for (const auto& u : used)
+      if (overlap(u.at, u.bytes, workspace, ws.total)) return PQ8_ERR_INVALID_ARGUMENT;
+  }
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
   if (fused) {
@@ -2619,7 +2633,7 @@ GroupNormPlan plan_group_norm(int size, bool vec, int rows, int windows, bool ra
     const long long all = std::max(rows, 1) * slabs;
     int c = 2;
     while (c < 8 && all * cols > 42000LL * c * sms) c *= 2;
-    return static_cast<int>(std::max((all + c * sms - 1) / (c * sms), least_rows));
+    return static_cast<int>(std::min(std::max((all + c * sms - 1) / (c * sms), least_rows), 1LL << 30));
   };
   g.block = block(g.slabs, g.slab * cg, 16);
   g.row_block = quantize ? block(1, channels, 8) : g.block;
@@ -2640,7 +2654,7 @@ int check_group_norm(const void* x, int type, const float* w, const float* b, co
                      const void* workspace) {
   if (offsets == nullptr && windows > 0 && rows % windows) return PQ8_ERR_UNSUPPORTED_SHAPE;
   const int size = type_size(type);
-  if (!(eps > 0.0) || !(eps < 1e30) || (act != PQ8_EPI_NONE && act != PQ8_EPI_RELU && act != PQ8_EPI_SILU))
+  if (!(eps >= 1e-30) || !(eps <= 1e30) || (act != PQ8_EPI_NONE && act != PQ8_EPI_RELU && act != PQ8_EPI_SILU))
     return PQ8_ERR_INVALID_ARGUMENT;
   if (rows == 0 || windows == 0) return PQ8_OK;
   if (x == nullptr || w == nullptr || b == nullptr || y == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
@@ -2654,12 +2668,17 @@ int check_group_norm(const void* x, int type, const float* w, const float* b, co
   return PQ8_OK;
 }
 
-// The workspace of the two-launch form: present, and no part of x or y.
-int check_norm_workspace(const GroupNormPlan& g, const void* ws, size_t ws_bytes, const void* x, size_t x_bytes,
-                         const void* y, size_t y_bytes) {
+// The workspace, where the plan has one: present, and no part of what else a call reads or writes.
+int check_norm_workspace(const GroupNormPlan& g, const void* ws, size_t ws_bytes, const GroupNormParams& p,
+                         size_t x_bytes, const void* y, size_t y_bytes, const float* scale) {
   if (g.total == 0) return PQ8_OK;
   if (ws == nullptr || ws_bytes < g.total) return PQ8_ERR_WORKSPACE;
-  return overlap(ws, g.total, x, x_bytes) || overlap(ws, g.total, y, y_bytes) ? PQ8_ERR_INVALID_ARGUMENT : PQ8_OK;
+  const size_t nw = static_cast<size_t>(p.channels) * 4;
+  const bool clash = overlap(ws, g.total, p.x, x_bytes) || overlap(ws, g.total, y, y_bytes) ||
+                     overlap(ws, g.total, p.w, nw) || overlap(ws, g.total, p.b, nw) ||
+                     overlap(ws, g.total, p.offsets, (static_cast<size_t>(p.windows) + 1) * 4) ||
+                     overlap(ws, g.total, scale, static_cast<size_t>(p.rows) * 4);
+  return clash ? PQ8_ERR_INVALID_ARGUMENT : PQ8_OK;
 }
 
 GroupNormParams group_norm_params(const GroupNormPlan& g, const void* x, const float* w, const float* b, int rows,
@@ -2755,12 +2774,12 @@ extern "C" int pq8_group_norm(const void* x, int type, const float* w, const flo
   if ((rc = device_state(&ds))) return rc;
   const GroupNormPlan g = plan_group_norm(type_size(type), aligned(x, 16) && aligned(y, 16), rows, windows,
                                           offsets != nullptr, channels, groups, false);
-  if ((rc = check_norm_workspace(g, workspace, workspace_bytes, x, bytes, y, bytes))) return rc;
+  GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
+  p.round_out = (flags & PQ8_FLAG_OUT_TF32) ? 1 : 0;
+  if ((rc = check_norm_workspace(g, workspace, workspace_bytes, p, bytes, y, bytes, nullptr))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
-    GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
-    p.round_out = (flags & PQ8_FLAG_OUT_TF32) ? 1 : 0;
     if (g.parts > 0)
       return g.units == kWhole
                  ? launch_group_norm_one<T, kWhole, false>(g, p, static_cast<T*>(y), GroupNormExtra{}, st)
@@ -2789,18 +2808,22 @@ extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, 
   rc = check_group_norm(x, type, w, b, q, q_bytes, rows, windows, offsets, channels, groups, eps, activation,
                         workspace);
   if (rc || rows == 0 || windows == 0) return rc;
-  if (scale == nullptr || overlap(scale, static_cast<size_t>(rows) * 4, x, x_bytes)) return PQ8_ERR_INVALID_ARGUMENT;
+  const size_t scale_bytes = static_cast<size_t>(rows) * 4, w_bytes = static_cast<size_t>(channels) * 4;
+  if (scale == nullptr || overlap(scale, scale_bytes, x, x_bytes) || overlap(scale, scale_bytes, q, q_bytes) ||
+      overlap(scale, scale_bytes, w, w_bytes) || overlap(scale, scale_bytes, b, w_bytes) ||
+      overlap(scale, scale_bytes, offsets, (static_cast<size_t>(windows) + 1) * 4))
+    return PQ8_ERR_INVALID_ARGUMENT;
   if (!aligned(q, 16) || !aligned(scale, 4)) return PQ8_ERR_MISALIGNED;
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
   const bool vec = aligned(x, 16) && aligned(w, 16) && aligned(b, 16);
   const GroupNormPlan g =
       plan_group_norm(type_size(type), vec, rows, windows, offsets != nullptr, channels, groups, true);
-  if ((rc = check_norm_workspace(g, workspace, workspace_bytes, x, x_bytes, q, q_bytes))) return rc;
+  const GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
+  if ((rc = check_norm_workspace(g, workspace, workspace_bytes, p, x_bytes, q, q_bytes, scale))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(type, [&](auto t) {
     using T = decltype(t);
-    const GroupNormParams p = group_norm_params(g, x, w, b, rows, windows, offsets, channels, groups, eps, activation);
     unsigned char* base = static_cast<unsigned char*>(workspace);
     if (g.parts > 0) {
       float* values = reinterpret_cast<float*>(base);

@@ -185,9 +185,10 @@ __device__ __forceinline__ void reduce_groups(const SlabShape<E>& sh, const Grou
   }
 }
 
+// Squares that left fp32's range (possible where values are over 2^60 apart) leave no statistics: NaN.
 __device__ __forceinline__ GroupStat group_stat(const GroupSum& t, double first, double n, double eps) {
   const double m = t.s / n;
-  return GroupStat{first + m, 1.0 / sqrt(fmax(t.q / n - m * m, 0.0) + eps)};
+  return GroupStat{first + m, t.q < INFINITY ? 1.0 / sqrt(fmax(t.q / n - m * m, 0.0) + eps) : NAN};
 }
 
 // The first value of slab group g in the window (0 for an empty window).

@@ -338,14 +338,16 @@ __device__ __forceinline__ void i8_finish(const uint32_t (&v)[E], const T (&rv)[
         g_prev = gate;
       } else {
         unpack2(mul2(pack2(a_prev, a), sigmoid2(pack2(g_prev, gate))), &out[j / 2 - 1], &out[j / 2]);
+        if (g_prev != g_prev) out[j / 2 - 1] = g_prev;  // sigmoid2 caps a NaN
+        if (gate != gate) out[j / 2] = gate;
       }
     } else {
       if constexpr (EPI == PQ8_EPI_RESIDUAL) z = fma2(pack2(alpha, alpha), z, pack2(to_f32(rv[j]), to_f32(rv[j + 1])));
       if constexpr (EPI == PQ8_EPI_SILU) z = mul2(z, sigmoid2(z));
       unpack2(z, &out[j], &out[j + 1]);
       if constexpr (EPI == PQ8_EPI_RELU) {
-        out[j] = fmaxf(out[j], 0.0f);
-        out[j + 1] = fmaxf(out[j + 1], 0.0f);
+        out[j] = relu_f32(out[j]);
+        out[j + 1] = relu_f32(out[j + 1]);
       }
     }
   }

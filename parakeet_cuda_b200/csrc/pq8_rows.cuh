@@ -124,7 +124,8 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
 // the special-function unit, which bounds epilogues with few other operations;
 // here the two share one reciprocal: 1 / d0 = d1 / (d0 d1). The exponent is
 // capped at 63 so that the product stays in range; below z = -43.7 the
-// result is 2^-63 instead of e^z, an absolute error under 2^-63.
+// result is 2^-63 instead of e^z, an absolute error under 2^-63. (A NaN is capped
+// too, so that it stays out of the other value's result.)
 __device__ __forceinline__ f32x2 sigmoid2(f32x2 z) {
   float e0, e1, r;
   unpack2(mul2(z, pack2(-1.44269504f, -1.44269504f)), &e0, &e1);
@@ -215,15 +216,21 @@ struct RowTeam {
   }
 };
 
+// max(z, 0) that a NaN passes (fmaxf would make it 0 and hide a bad row).
+__device__ __forceinline__ float relu_f32(float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
+  return r;
+}
 __device__ __forceinline__ double act_f64(double z, int epi) {
-  if (epi == PQ8_EPI_RELU) return z > 0.0 ? z : 0.0;
+  if (epi == PQ8_EPI_RELU) return z < 0.0 ? 0.0 : z;
   if (epi == PQ8_EPI_SILU) return z / (1.0 + exp(-z));
   return z;
 }
 // SiLU by the fast exponential and quotient: within 4 x 2^-23 |y| + 2^-23 of the
 // exact one (the exponential's error grows with |z|, where e^z shrinks faster).
 __device__ __forceinline__ float act_f32(float z, int epi) {
-  if (epi == PQ8_EPI_RELU) return fmaxf(z, 0.0f);
+  if (epi == PQ8_EPI_RELU) return relu_f32(z);
   if (epi == PQ8_EPI_SILU) return __fdividef(z, 1.0f + __expf(-z));
   return z;
 }

@@ -60,7 +60,7 @@ ELEMENT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat1
 
 class _Int8Rows:
     """A dense int8 matrix with a float32 scale per row, checked once when it is made."""
-    __slots__ = ('_q', '_scale', 'n', 'k', 'device', 'q_ptr', 'scale_ptr')
+    __slots__ = ('_q', '_scale', 'n', 'k', 'device')
     q = property(lambda self: self._q)
     scale = property(lambda self: self._scale)
 
@@ -75,7 +75,13 @@ class _Int8Rows:
         self.device = q.device
         if scale.device != self.device:
             raise ValueError(f'q is on {q.device}, scale on {scale.device}')
-        self._q, self._scale, self.q_ptr, self.scale_ptr = q, scale, q.data_ptr(), scale.data_ptr()
+        self._q, self._scale = q, scale
+
+    def pointers(self) -> tuple[int, int]:
+        """Addresses of the integers and the scales, as they are now."""
+        if self._q.shape != (self.n, self.k) or self._scale.shape != (self.n,):
+            raise ValueError('the integers or scales have changed their shape')
+        return self._q.data_ptr(), self._scale.data_ptr()
 
 
 class Int8Weight(_Int8Rows):
@@ -331,6 +337,8 @@ class Runtime:
             raise ValueError(f'x must be a float32, float16 or bfloat16 matrix on {self.device}, got {x.dtype} '
                              f'{tuple(x.shape)} on {x.device}')
         rows, width = x.shape
+        if rows > 1 << 30:
+            raise ValueError(f'at most 2^30 rows a call, got {rows}')
         ld, step = x.stride()
         if rows <= 1:
             ld = width
@@ -358,12 +366,11 @@ class Runtime:
         out = QuantizedRows(torch.empty(rows, width, dtype=torch.int8, device=self.device),
                             torch.empty(rows, dtype=torch.float32, device=self.device))
         if norm is None:
-            self._enqueue('pq8_quantize_rows', x.data_ptr(), kind, ld, out.q_ptr, out.scale_ptr, rows, width)
+            self._enqueue('pq8_quantize_rows', x.data_ptr(), kind, ld, *out.pointers(), rows, width)
         else:
             w = self._check(norm[0], 'the norm weight', torch.float32, (width,))
             b = self._check(norm[1], 'the norm bias', torch.float32, (width,))
-            self._enqueue('pq8_layer_norm_quantize', x.data_ptr(), kind, ld, w, b, out.q_ptr, out.scale_ptr, rows,
-                          width)
+            self._enqueue('pq8_layer_norm_quantize', x.data_ptr(), kind, ld, w, b, *out.pointers(), rows, width)
         return out
 
     def int8_weight(self, w) -> Int8Weight:
@@ -414,8 +421,7 @@ class Runtime:
         b = None if bias is None else self._check(bias, 'bias', torch.float32, (n,))
         r = None if resid is None else self._check(resid, 'resid', out.dtype, (rows, cols))
         if quantized:
-            self._enqueue('pq8_gemm_i8', w.q_ptr, w.scale_ptr, x.q_ptr, x.scale_ptr, y, y_kind, b, r, rows, n, k,
-                          epilogue, alpha)
+            self._enqueue('pq8_gemm_i8', *w.pointers(), *x.pointers(), y, y_kind, b, r, rows, n, k, epilogue, alpha)
             return out
         g = h = None
         if norm is not None:
@@ -425,17 +431,20 @@ class Runtime:
         at = x.data_ptr()
         need = pq8.linear_i8_scratch(rows, k, at | (0 if rows <= 1 else ld * x.element_size()) | (g or 0) | (h or 0))
         scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        self._enqueue('pq8_linear_i8', w.q_ptr, w.scale_ptr, at, kind, ld, g, h, y, y_kind, b, r, rows, n, k,
+        self._enqueue('pq8_linear_i8', *w.pointers(), at, kind, ld, g, h, y, y_kind, b, r, rows, n, k,
                       epilogue, alpha, _ptr(scratch), need)
         return out
 
     # -- group norm --------------------------------------------------------------
-    def _check_group_norm(self, x, weight, bias, windows, offsets):
+    def _check_group_norm(self, x, weight, bias, groups, windows, offsets):
         """(rows, channels, type code, addresses of x, weight, bias and offsets)."""
         kind = ELEMENT_TYPES.get(x.dtype)
         if kind is None or x.dim() != 2:
             raise ValueError(f'x must be a float32, float16 or bfloat16 matrix, got {x.dtype} {tuple(x.shape)}')
         rows, channels = x.shape
+        if rows > 1 << 30 or not 0 < groups <= channels or windows > 1 << 24:
+            raise ValueError(f'{rows} rows in {windows} windows, {channels} channels in {groups} groups: at most 2^30 rows '
+                             'in 2^24 windows, and a group has a channel')
         at = (self._check(x, 'x', x.dtype, x.shape), self._check(weight, 'weight', torch.float32, (channels,)),
               self._check(bias, 'bias', torch.float32, (channels,)))
         off = None
@@ -452,7 +461,7 @@ class Runtime:
         [rows, channels] in ``windows`` windows of equal length, or of the rows ``offsets[i]`` to
         ``offsets[i + 1] - 1`` (int32 on the device, ``windows + 1`` of them). Rows in no window are
         not written: ``out`` keeps what it held, and a new tensor has nothing there."""
-        rows, channels, kind, at, off = self._check_group_norm(x, weight, bias, windows, offsets)
+        rows, channels, kind, at, off = self._check_group_norm(x, weight, bias, groups, windows, offsets)
         if out is None:
             out = torch.empty_like(x)
             y = out.data_ptr()
@@ -469,13 +478,13 @@ class Runtime:
                             eps: float = 1e-5, epilogue: int = EPI_NONE) -> QuantizedRows:
         """``group_norm``, its rows quantised as ``quantize_rows`` does, for ``linear_i8``. Rows in no window
         have no values and no scale."""
-        rows, channels, kind, at, off = self._check_group_norm(x, weight, bias, windows, offsets)
+        rows, channels, kind, at, off = self._check_group_norm(x, weight, bias, groups, windows, offsets)
         out = QuantizedRows(torch.empty(rows, channels, dtype=torch.int8, device=self.device),
                             torch.empty(rows, dtype=torch.float32, device=self.device))
         need = self.lib.group_norm_workspace_size(kind, rows, windows, channels, groups, off is not None, True,
                                                   not (at[0] | at[1] | at[2]) & 15)
         scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._enqueue('pq8_group_norm_quantize', at[0], kind, at[1], at[2], out.q_ptr, out.scale_ptr, rows, windows,
+        self._enqueue('pq8_group_norm_quantize', at[0], kind, at[1], at[2], *out.pointers(), rows, windows,
                       off, channels, groups, eps, epilogue, _ptr(scratch), need)
         return out
 

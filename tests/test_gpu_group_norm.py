@@ -256,3 +256,42 @@ def test_group_norm_refuses(rt):
         with pytest.raises(pq8.PQ8Error):
             f()
     assert rt.group_norm(x[:0], w, b, 4).shape == (0, 64)
+
+
+def test_group_norm_bad_values_pass_every_activation(rt):
+    """An infinity or a NaN makes its group NaN through every activation; values too far apart for squares in
+    fp32 give NaN or the right result; other groups and windows keep their bits. Quantised, a bad value takes its rows' scales."""
+    for channels, groups, dtype in ((64, 4, torch.float32), (1000, 8, torch.float16), (35, 5, torch.float32)):
+        x, w, b = inputs(15, 60, channels, dtype)
+        cg = channels // groups
+        values = [float('inf'), float('nan')] + ([3e38, 1e30] if dtype == torch.float32 else [])
+        for name, act in ACTS.items():
+            clean = rt.group_norm(x, w, b, groups, windows=3, epilogue=act)
+            for value in values:
+                y = x.clone()
+                y[25, cg + 1] = value  # window 1, group 1
+                got = rt.group_norm(y, w, b, groups, windows=3, epilogue=act)
+                nan = torch.isnan(got[20:40, cg:2 * cg])
+                assert nan.all() if not np.isfinite(value) else nan.all() or not nan.any(), (channels, act, value)
+                if not nan.any():
+                    check(got, y, w, b, groups, [0, 20, 40, 60], name)
+                got[20:40, cg:2 * cg] = clean[20:40, cg:2 * cg]
+                assert torch.equal(got, clean)
+    x, w, b = inputs(16, 60, 64, torch.float32)
+    for act in ACTS.values():
+        clean = rt.group_norm_quantize(x, w, b, 4, windows=3, epilogue=act)
+        for value in (float('inf'), float('nan')):
+            y = x.clone()
+            y[25, 17] = value
+            got = rt.group_norm_quantize(y, w, b, 4, windows=3, epilogue=act)
+            assert torch.isnan(got.scale[20:40]).all() and not got.q[20:40].any()
+            assert torch.equal(got.scale[:20], clean.scale[:20]) and torch.equal(got.q[40:], clean.q[40:])
+
+
+def test_group_norm_refuses_sizes(rt):
+    x, w, b = torch.zeros(12, 64, device='cuda'), torch.ones(64, device='cuda'), torch.zeros(64, device='cuda')
+    for groups in (0, -4, 128, (1 << 32) + 4):
+        with pytest.raises(ValueError):
+            rt.group_norm(x, w, b, groups)
+    with pytest.raises(ValueError):
+        rt.group_norm(x[:0], w, b, 4, windows=1 << 32)

@@ -10,7 +10,10 @@ quotient: under 8 x 2^-24 of the result) and pass the error of z on with a slope
 rounding is half a step of its type.
 """
 import ctypes as C
+import subprocess
+import sys
 from fractions import Fraction
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -356,3 +359,100 @@ def test_linear_i8_refuses(rt):
             f()
     assert rt.linear_i8(x[:0], w8).shape == (0, 32)
     assert rt.linear_i8(rt.quantize_rows(x[:0]), w8).shape == (0, 32)
+
+
+def test_linear_i8_nan_passes_every_epilogue(rt):
+    """A bad row, a bad channel and a bad gate reach the output through every activation, and nothing else."""
+    rng = np.random.default_rng(12)
+    n, k = 192, 256
+    w, t = weights(rng, n, k)
+    bad_t = t.copy()
+    bad_t[100] = np.nan  # for the GLU: the gate of channel 4
+    for m in (3, 20, 300):
+        x = rng.normal(size=(m, k)).astype(np.float32)
+        x[1, 7] = np.inf
+        for epi in (EPI_NONE, EPI_RELU, EPI_SILU, EPI_GLU):
+            clean = rt.linear_i8(dev(np.delete(x, 1, 0)), Int8Weight(dev(w), dev(t)), epilogue=epi)
+            got = rt.linear_i8(dev(x), Int8Weight(dev(w), dev(bad_t)), epilogue=epi)
+            assert torch.isnan(got[1]).all()
+            col = 4 if epi == EPI_GLU else 100
+            assert torch.isnan(got[:, col]).all()
+            rest = torch.cat([got[:1], got[2:]])
+            keep = [j for j in range(got.shape[1]) if j != col]
+            if epi in (EPI_NONE, EPI_RELU):
+                assert torch.equal(rest[:, keep], clean[:, keep])
+            else:
+                # two tokens' sigmoids share one reciprocal, and without the bad row other tokens are
+                # neighbours: each side is within 8 U |y| of the same z's activation (module docstring)
+                a, b = f64(rest[:, keep]), f64(clean[:, keep])
+                assert (np.abs(a - b) <= 8 * U * (np.abs(a) + np.abs(b)) + 2.0 ** -62).all()
+
+
+def test_int8_weight_that_changed_its_shape(rt):
+    """The weight's storage is looked up at the call: a replaced one is used, a smaller one refused."""
+    w8 = Int8Weight(torch.ones(32, 64, dtype=torch.int8, device='cuda'), torch.ones(32, device='cuda'))
+    x = torch.ones(9, 64, device='cuda')
+    a = rt.linear_i8(x, w8)
+    w8.q.data = torch.full((32, 64), 2, dtype=torch.int8, device='cuda')
+    assert torch.equal(rt.linear_i8(x, w8), 2 * a)
+    w8.q.data = torch.ones(16, 64, dtype=torch.int8, device='cuda')
+    with pytest.raises(ValueError):
+        rt.linear_i8(x, w8)
+
+
+FIRST_CALL = """
+import torch
+from parakeet_cuda_b200.runtime import Int8Weight, Runtime
+rt = Runtime(0)
+torch.manual_seed(0)
+w8 = Int8Weight(torch.randint(-127, 128, (512, 4096), dtype=torch.int8, device='cuda'), torch.rand(512, device='cuda'))
+gw, gb = torch.rand(4096, device='cuda'), torch.rand(4096, device='cuda')
+xs = [torch.randn(m, 4096, device='cuda') for m in (1, 5, 60, 400, 2500)]
+def step():
+    out = [rt.linear_i8(x, w8, norm=(gw, gb)) for x in xs]
+    for x in xs:
+        out.append(rt.group_norm(x, gw, gb, 32))
+        out.append(rt.group_norm_quantize(x, gw, gb, 32).scale)
+    return out
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+assert rt.device_status() == 0
+print('same')
+"""
+
+
+def test_first_calls_captured():
+    """A process whose first calls are captured: per-device state is made under capture, same bits as eager."""
+    root = Path(__file__).resolve().parent.parent
+    run = subprocess.run([sys.executable, '-c', FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and 'same' in run.stdout, run.stderr[-2000:]
+
+
+def test_two_graphs_in_flight(rt):
+    """Two captured graphs replayed on two streams at once, each with its own scratch."""
+    rng = np.random.default_rng(13)
+    w8 = rt.int8_weight(dev(rng.normal(size=(1024, 1024)).astype(np.float32)))
+    g, b = dev(rng.normal(size=1024).astype(np.float32)), dev(rng.normal(size=1024).astype(np.float32))
+    xs = [dev(rng.normal(size=(700, 1024)).astype(np.float32)) for _ in range(2)]
+    made = []
+    for x in xs:
+        want = rt.linear_i8(rt.group_norm_quantize(x, g, b, 4), w8, resid=x, epilogue=EPI_RESIDUAL)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = x
+            for _ in range(4):
+                y = rt.linear_i8(rt.group_norm_quantize(x, g, b, 4), w8, resid=x, epilogue=EPI_RESIDUAL)
+        made.append((graph, y, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for graph, _, _, st in made:
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, y, want, _ in made:
+        assert torch.equal(y, want)

@@ -152,3 +152,33 @@ def test_oracle_quantize_ties_and_empty_rows():
     assert q[0].tolist() == [127, 0, 2, 2, 0, -2, 3, -4] and s[0] == 1.0
     assert not q[1].any() and s[1] == 0
     assert not q[2].any() and np.isnan(s[2])
+
+
+def test_int8_refusals_at_the_edges(lib):
+    """Sizes past 2^30, and outputs or workspaces inside what the call still has to read."""
+    many = (1 << 30) + 1
+    assert rows(lib, rows=many) == pq8.ERR_UNSUPPORTED_SHAPE
+    assert gemm(lib, m=many) == gemm(lib, n=many) == pq8.ERR_UNSUPPORTED_SHAPE
+    assert linear(lib, m=many) == pq8.ERR_UNSUPPORTED_SHAPE
+    assert code(lib, 'pq8_linear_i8_workspace_size', many, 64, C.byref(C.c_size_t())) == pq8.ERR_UNSUPPORTED_SHAPE
+    assert rows(lib, s=Q + 64) == pq8.ERR_INVALID_ARGUMENT  # scales inside q
+    for q, s in ((W, S), (B, S), (Q, W), (Q, B)):
+        assert code(lib, 'pq8_layer_norm_quantize', X, 0, 64, W, B, q, s, 4, 64, None) == pq8.ERR_INVALID_ARGUMENT
+    assert linear(lib, y=B, nw=W + 64, nb=B) == pq8.ERR_INVALID_ARGUMENT  # y over the norm's bias
+    for at in (W, S, B):  # the workspace over the weights, their scales, the norm
+        assert linear(lib, m=9, ws=at, nw=B, nb=B + 4096) == pq8.ERR_INVALID_ARGUMENT, at
+    for bias, resid in ((WS + 64, Y), (None, WS + 64)):
+        assert code(lib, 'pq8_linear_i8', W, S, X, 0, 64, None, None, Y, 0, bias, resid, 9, 64, 64, pq8.EPI_RESIDUAL,
+                    1.0, WS, BIG, None) == pq8.ERR_INVALID_ARGUMENT
+    for eps in (9e-31, 1.1e30):
+        assert norm(lib, eps=eps) == pq8.ERR_INVALID_ARGUMENT
+
+
+def test_group_norm_workspace_sizes(lib):
+    """The largest shapes that the size query takes: no size leaves 64 bits, none is missing."""
+    for rows_, windows, c, g in ((1 << 30, 1, 16384, 4096), (1 << 30, 1, 16384, 1), (1 << 30, 1 << 24, 16, 16), (1, 1, 16, 16)):
+        for quantize in (False, True):
+            for ragged in (False, True):
+                need = lib.group_norm_workspace_size(2, rows_, windows, c, g, ragged, quantize)
+                assert 0 <= need < 1 << 48, (rows_, windows, c, g)
+                assert need or not quantize
