@@ -16,6 +16,14 @@
 // cluster's CTAs exchange their sums, and each normalises what it holds.
 // Otherwise (long windows of wide groups, rows that 16-byte loads do not fit)
 // partial sums go through a workspace and a second launch reads x again.
+//
+// Measured (bytes of x and y over the time): 8 x 375 x 1024 fp32, 32 groups,
+// one launch 9.7 us (2.5 TB/s: one wave of CTAs that load, sum, meet and store in
+// turn, 14,000 cycles), 64 windows 46.5 us (4.2 TB/s); 64 x 375 x 1024 bf16 in one
+// group 40.8 us (2.4 TB/s). There two CTAs an SM take 34,000 cycles a wave: 11,000
+// to load, 4000 to sum, 3000 to exchange, 14,000 to normalise and store (8000
+// without SiLU: the special-function unit). 13 ragged windows of 7969 x 1000 fp16
+// in two launches 22 us. Quantised, 8 x 375 x 1024: 19 us, of which the second launch 8.
 #pragma once
 
 #include "pq8_rows.cuh"

@@ -38,7 +38,11 @@ __device__ __forceinline__ float i8_scaled(int acc, float s, float t, float b) {
 // lane every 32nd 16-byte chunk; the lanes' sums meet in one reduction per
 // output. With FUSED the tokens arrive in floating point and every CTA
 // quantises them for itself into shared memory (the same few KB from L2 for
-// all of them), which saves the launch and the round trip of a pass of its own.
+// all of them), which saves the launch and the round trip of a pass of its own:
+// 1 x 1024 x 4096 (tokens x K x channels) from fp32 in 2.6 us against 5.0 in two
+// launches, 8 x 640 x 8198 in 5.6 against 11.8 (in a graph). Product alone: 1 x
+// 1024 x 4096 2.0 us (2.1 TB/s of weights: launch and one round trip to memory),
+// 8 x 640 x 8198 4.2 (1.3 TB/s: eight dp4a sums per weight word).
 constexpr int kI8GemvThreads = 256;
 constexpr int kI8GemvMaxM = 8;
 
@@ -205,6 +209,12 @@ __global__ void __launch_bounds__(kI8GemvThreads, 2) i8_gemv_kernel(const I8Para
 // shared memory, CTA s finishing rows [s, s + 1) BN / S of the tile.
 //
 // Two accumulators let the next tile's products run under a tile's epilogue.
+//
+// Measured: 8192^3 350 us (3.14e15 operations/s, 0.93 of the rate taken for 8 bits:
+// twice the bf16 product's); 24,000 x 1024 x 4096 with SiLU to bf16 97.5 us (2.07e15;
+// the chip is at its power limit there, 990 W at 1.5 GHz, and the products
+// alone take 66); 3000 x 4096 x 1024 17.6 us (one wave and a bit of pairs);
+// 375 x 1024 x 2048 GLU 5.6 us (3 us of launch, set-up and first loads).
 //
 // Warps: 0 and 2 TMA producers, 1 MMA issuer (and tensor-memory owner), 3
 // scheduler of the MMA issuer, 4 on: epilogue.

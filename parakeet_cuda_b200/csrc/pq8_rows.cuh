@@ -26,7 +26,7 @@
 namespace pq8 {
 
 // ---------------------------------------------------------------------------
-// Element types (PQ8_F32, PQ8_F16, PQ8_BF16)
+// Element types (PQ8_TYPE_F32, PQ8_TYPE_F16, PQ8_TYPE_BF16)
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>
@@ -474,7 +474,8 @@ __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, con
   float s = top / 127.0f;
   if constexpr (!Src::kExact) {
     if (top < INFINITY) {
-      // the values that may be the largest, exactly
+      // the values that may be the largest, exactly (looked for only in chunks that
+      // reach the bound; whole chunks in fp64 took 35 us for 24,000 x 1024 bf16)
       const float least = top - 2.5f * src.error(top);
       double t64 = 0.0;
       if (mine >= least) {
@@ -482,11 +483,13 @@ __device__ __forceinline__ float quantize_row(Src src, int width, int8_t* q, con
           uint32_t found = 0;
 #pragma unroll
           for (int j = 0; j < N; ++j)
-            if (has(tid + j * kThreads) && chunk_top[j] >= least) found |= 1u << j;
+            if (has(tid + j * kThreads) && chunk_top[j] >= least) {
+#pragma unroll
+              for (int i = 0; i < E; ++i) found |= fabsf(v[j][i]) >= least ? 1u << (j * E + i) : 0u;
+            }
           for (; found; found &= found - 1) {
-            const int col = (tid + (__ffs(found) - 1) * kThreads) * E;
-#pragma unroll 1
-            for (int i = 0; i < E; ++i) t64 = fmax(t64, ::fabs(src.exact(col + i)));
+            const int bit = __ffs(found) - 1;
+            t64 = fmax(t64, ::fabs(src.exact((tid + (bit / E) * kThreads) * E + bit % E)));
           }
         } else {
           columns([&](float u) { return fabsf(u) >= least; },
@@ -549,7 +552,10 @@ constexpr int kRowThreads = 256;
 // a team of WARPS warps: a warp per row up to 1024 columns, the CTA's eight
 // warps up to 8192 (the row stays in registers in both), and past that, or
 // where 16-byte loads do not fit, the CTA reads the row again in each pass.
-// NORM: LayerNorm first.
+// NORM: LayerNorm first. Bound by HBM for fp32 rows as they are (24,000 x
+// 1024: 19.5 us, 6.3 TB/s), by instruction issue otherwise: bf16 18 us (the same
+// instructions over half the bytes), after a LayerNorm 30 us fp32, 29 us bf16 (fp64
+// sums, and the long chain of reductions of a row, at 24 warps an SM).
 template <typename T, int CHUNKS, int WARPS, bool FULL, bool NORM, bool VEC>
 __global__ void __launch_bounds__(kRowThreads, NORM ? 3 : 4)
     quantize_rows_kernel(const T* __restrict__ x, long long ld, const float* __restrict__ w,

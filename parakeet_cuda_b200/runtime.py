@@ -61,8 +61,9 @@ ELEMENT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat1
 class _Int8Rows:
     """A dense int8 matrix with a float32 scale per row, checked once when it is made."""
     __slots__ = ('_q', '_scale', 'n', 'k', 'device')
-    q = property(lambda self: self._q)
-    scale = property(lambda self: self._scale)
+    # aliases: their memory can be written through them, but not exchanged
+    q = property(lambda self: self._q.detach())
+    scale = property(lambda self: self._scale.detach())
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
         if q.dtype != torch.int8 or q.dim() != 2 or not q.is_contiguous():
@@ -75,12 +76,10 @@ class _Int8Rows:
         self.device = q.device
         if scale.device != self.device:
             raise ValueError(f'q is on {q.device}, scale on {scale.device}')
-        self._q, self._scale = q, scale
+        self._q, self._scale = q.detach(), scale.detach()
 
     def pointers(self) -> tuple[int, int]:
         """Addresses of the integers and the scales, as they are now."""
-        if self._q.shape != (self.n, self.k) or self._scale.shape != (self.n,):
-            raise ValueError('the integers or scales have changed their shape')
         return self._q.data_ptr(), self._scale.data_ptr()
 
 
