@@ -295,3 +295,23 @@ def test_group_norm_refuses_sizes(rt):
             rt.group_norm(x, w, b, groups)
     with pytest.raises(ValueError):
         rt.group_norm(x[:0], w, b, 4, windows=1 << 32)
+
+
+def test_group_norm_past_32_bit_offsets(rt):
+    """More than 2^31 values, windows of equal and of unequal lengths: the last window is right."""
+    torch.manual_seed(17)
+    channels, t = 1024, 3000
+    windows = (1 << 31) // (channels * t) + 2
+    x = torch.randn(windows * t, channels, device='cuda', dtype=torch.bfloat16)
+    _, w, b = inputs(17, 1, channels, torch.float32)
+    last = x[(windows - 1) * t:].clone()
+    for groups in (32, 1):  # one launch, two launches
+        y = rt.group_norm(x, w, b, groups, windows=windows, epilogue=EPI_SILU)
+        check(y[(windows - 1) * t:], last, w, b, groups, [0, t], 'silu')
+        off = torch.tensor([0, 5, windows * t - 77, windows * t], dtype=torch.int32, device='cuda')
+        rt.group_norm(x, w, b, groups, windows=3, offsets=off, epilogue=EPI_SILU, out=y)
+        check(y[-77:], x[-77:], w, b, groups, [0, 77], 'silu')
+    del y
+    got = rt.group_norm_quantize(x, w, b, 32, windows=windows, epilogue=EPI_SILU)
+    alone = rt.group_norm_quantize(last, w, b, 32, epilogue=EPI_SILU)
+    assert torch.equal(got.scale[(windows - 1) * t:], alone.scale) and torch.equal(got.q[(windows - 1) * t:], alone.q)

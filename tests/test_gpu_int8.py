@@ -461,3 +461,31 @@ def test_two_graphs_in_flight(rt):
     torch.cuda.synchronize()
     for _, y, want, _ in made:
         assert torch.equal(y, want)
+
+
+def test_past_32_bit_offsets(rt):
+    """Tokens, integers and outputs of more than 2^31 elements: the last rows are what they are alone."""
+    rng = np.random.default_rng(14)
+    torch.manual_seed(14)
+    w, t = weights(rng, 8192, 64)
+    w8 = Int8Weight(dev(w), dev(t))
+    m = (1 << 31) // 8192 + 500
+    x = torch.randn(m, 64, device='cuda')
+    y = rt.linear_i8(x, w8, out_dtype=torch.bfloat16)
+    for part in (slice(0, 300), slice(m - 300, m)):
+        assert torch.equal(y[part], rt.linear_i8(x[part], w8, out_dtype=torch.bfloat16))
+    del y
+    m = (1 << 31) // 4096 + 70
+    x = torch.randn(m, 4096, device='cuda', dtype=torch.float16)
+    got = rt.quantize_rows(x)
+    alone = rt.quantize_rows(x[m - 90:])
+    assert torch.equal(got.q[m - 90:], alone.q) and torch.equal(got.scale[m - 90:], alone.scale)
+    w, t = weights(rng, 48, 4096)
+    w8 = Int8Weight(dev(w), dev(t))
+    y, z = rt.linear_i8(got, w8), rt.linear_i8(alone, w8)
+    assert torch.equal(y[m - 90:], z)
+    far = torch.empty_strided((9, 64), (1 << 29, 1), dtype=torch.float16, device='cuda')  # rows 1 GB apart
+    far.copy_(x[:9, :64])
+    near = rt.quantize_rows(x[:9, :64].contiguous())
+    got = rt.quantize_rows(far)
+    assert torch.equal(got.q, near.q) and torch.equal(got.scale, near.scale)
