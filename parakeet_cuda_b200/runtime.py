@@ -61,9 +61,8 @@ ELEMENT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat1
 class _Int8Rows:
     """A dense int8 matrix with a float32 scale per row, checked once when it is made."""
     __slots__ = ('_q', '_scale', 'n', 'k', 'device')
-    # aliases: their memory can be written through them, but not exchanged
-    q = property(lambda self: self._q.detach())
-    scale = property(lambda self: self._scale.detach())
+    q = property(lambda self: self._q)
+    scale = property(lambda self: self._scale)
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
         if q.dtype != torch.int8 or q.dim() != 2 or not q.is_contiguous():
@@ -76,11 +75,14 @@ class _Int8Rows:
         self.device = q.device
         if scale.device != self.device:
             raise ValueError(f'q is on {q.device}, scale on {scale.device}')
-        self._q, self._scale = q.detach(), scale.detach()
+        self._q, self._scale = q, scale
 
     def pointers(self) -> tuple[int, int]:
-        """Addresses of the integers and the scales, as they are now."""
-        return self._q.data_ptr(), self._scale.data_ptr()
+        """Addresses of the integers and the scales, as they are now (a tensor can be given other memory)."""
+        q, scale = self._q, self._scale
+        if q.nbytes != self.n * self.k or scale.nbytes != 4 * self.n or not (q.is_contiguous() and scale.is_contiguous()):
+            raise ValueError('the integers or the scales have changed their shape or type')
+        return q.data_ptr(), scale.data_ptr()
 
 
 class Int8Weight(_Int8Rows):

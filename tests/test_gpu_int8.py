@@ -388,21 +388,24 @@ def test_linear_i8_nan_passes_every_epilogue(rt):
                 assert (np.abs(a - b) <= 8 * U * (np.abs(a) + np.abs(b)) + 2.0 ** -62).all()
 
 
-def test_int8_weight_memory_is_its_own(rt):
-    """A weight can be written in place; giving a tensor it was made of, or one it hands out, other memory or
-    another shape does not reach it."""
+def test_int8_weight_whose_memory_changes(rt):
+    """A weight can be written in place or given other memory of its size; memory of another is refused."""
     q, s = torch.ones(32, 64, dtype=torch.int8, device='cuda'), torch.ones(32, device='cuda')
     w8 = Int8Weight(q, s)
     x = torch.ones(9, 64, device='cuda')
     a = rt.linear_i8(x, w8)
     w8.q.fill_(2)
     assert torch.equal(rt.linear_i8(x, w8), 2 * a)
-    for t in (q, w8.q):
-        t.data = torch.ones(1, 64, dtype=torch.int8, device='cuda').expand(32, 64)
-    s.data = torch.zeros(1, device='cuda')
-    del q, s, t
-    torch.cuda.empty_cache()
-    assert torch.equal(rt.linear_i8(x, w8), 2 * a)
+    q.data = torch.full((32, 64), 3, dtype=torch.int8, device='cuda')
+    assert torch.equal(rt.linear_i8(x, w8), 3 * a)
+    for bad in (torch.ones(16, 64, dtype=torch.int8, device='cuda'), torch.ones(1, 64, dtype=torch.int8, device='cuda').expand(32, 64)):
+        q.data = bad
+        with pytest.raises(ValueError):
+            rt.linear_i8(x, w8)
+    q.data = torch.ones(32, 64, dtype=torch.int8, device='cuda')
+    s.data = torch.ones(31, device='cuda')
+    with pytest.raises(ValueError):
+        rt.linear_i8(x, w8)
 
 
 FIRST_CALL = """
