@@ -41,7 +41,7 @@ def stale() -> bool:
     if not LIB.exists():
         return True
     t = LIB.stat().st_mtime
-    deps = sources() + sorted(CSRC.glob('*.cuh')) + [INCLUDE / 'pq8.h']
+    deps = sources() + sorted(CSRC.glob('*.cuh')) + sorted(CSRC.glob('*.h')) + [INCLUDE / 'pq8.h']
     return any(p.stat().st_mtime > t for p in deps)
 
 

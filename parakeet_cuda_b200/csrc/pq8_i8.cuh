@@ -11,6 +11,7 @@
 #include <cuda.h>
 
 #include "pq8_rows.cuh"
+#include "pq8_schedule.h"
 
 namespace pq8 {
 
@@ -441,6 +442,7 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR>::kThreads, 1)
   const int my_split = split ? static_cast<int>(cluster_rank()) : 0;
   const int per_split = (g.k_blocks + S - 1) / S;
   const int kb0 = my_split * per_split, kb1 = min(kb0 + per_split, g.k_blocks);
+  const ScheduleRange mine{tile0, num_tiles, tile_step, kb0, kb1};
 
   if (warp == 0 || warp == 2) {
     // ------------------------------------------------------------ producers
@@ -498,60 +500,53 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR>::kThreads, 1)
     // through a named barrier: a shared-memory access by the warp that
     // issues tcgen05.mma is held behind the products it has queued, so its own
     // waits would drain the tensor pipe at every K block (128 x 16384 x 1024 in
-    // tiles of 32: 39 us with the MMA warp waiting for itself, 35 so). Both warps meet the same
-    // number of times; the barrier carries the flag to stop.
+    // tiles of 32: 39 us with the MMA warp waiting for itself, 35 so). A wait that gives up is
+    // told to the MMA warp in the next meeting (pq8_schedule.h).
     if (leader) {
-      bool bad = false;
-      int local = 0;
       Ring<STAGES> ring;
-      for (int tile = tile0; tile < num_tiles && !bad; tile += tile_step, ++local) {
-        if (lane == 0) bad = !mbar_wait(&acc_empty[local & 1], ((local >> 1) & 1) ^ 1, abort_flag, status);
-        for (int kb = kb0; kb < kb1 && !bad; kb += C::kRelease) {
-          const int n = min(C::kRelease, kb1 - kb);
-          if (lane == 0)
-            for (int b = 0; b < n && !bad; ++b, ring.advance(1))
-              bad = !mbar_wait(&full[ring.idx], ring.phase, abort_flag, status);
-          bad = __shfl_sync(0xffffffffu, bad, 0);
-          bad = rendezvous_or(1, bad);
-        }
-      }
+      schedule_products(
+          mine, C::kRelease,
+          [&](int local) {  // lane 0's answer; landed() makes it the warp's
+            return lane != 0 || mbar_wait(&acc_empty[local & 1], ((local >> 1) & 1) ^ 1, abort_flag, status);
+          },
+          [&](int n, bool ok) {
+            if (lane == 0)
+              for (int b = 0; b < n && ok; ++b, ring.advance(1))
+                ok = mbar_wait(&full[ring.idx], ring.phase, abort_flag, status);
+            return __shfl_sync(0xffffffffu, ok, 0) != 0;
+          },
+          [&](bool bad) { return rendezvous_or(1, bad); });
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (leader) {
       constexpr uint32_t idesc = idesc_i8(128 * C::kCtas, BN);
       const uint64_t desc0 = smem_desc_sw128(smem_addr(smem));
-      bool stop = false, issued = false;
-      int local = 0;
+      bool issued = false;
       Ring<STAGES> ring;
-      for (int tile = tile0; tile < num_tiles && !stop; tile += tile_step, ++local) {
-        const int acc = local & 1;
-        const uint32_t d = tmem + acc * BN;
-        for (int kb = kb0; kb < kb1; kb += C::kRelease) {
-          const int n = min(C::kRelease, kb1 - kb);
-          if (rendezvous_or(1, false)) {  // the scheduler gave up
-            stop = true;
-            break;
-          }
-          tc_fence_after();
-          if (lane == 0) {
-            for (int b = 0; b < n; ++b, ring.advance(1)) {
-              const uint64_t ad = desc0 + ring.idx * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
+      const bool stop = issue_products(
+          mine, C::kRelease, [&](bool bad) { return rendezvous_or(1, bad); },
+          [&](int local, int kb, int n) {
+            const int acc = local & 1;
+            const uint32_t d = tmem + acc * BN;
+            tc_fence_after();
+            if (lane == 0) {
+              for (int b = 0; b < n; ++b, ring.advance(1)) {
+                const uint64_t ad = desc0 + ring.idx * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                mma_i8<PAIR>(d, ad + 2 * j, bd + 2 * j, idesc, (kb + b > kb0 || j > 0) ? 1u : 0u);
-              if constexpr (PAIR) mma_commit_pair(&empty[ring.idx], 0x3);
-              else mma_commit(&empty[ring.idx]);
+                for (int j = 0; j < 4; ++j)
+                  mma_i8<PAIR>(d, ad + 2 * j, bd + 2 * j, idesc, (kb + b > kb0 || j > 0) ? 1u : 0u);
+                if constexpr (PAIR) mma_commit_pair(&empty[ring.idx], 0x3);
+                else mma_commit(&empty[ring.idx]);
+              }
+              if (kb + n == kb1) {
+                if constexpr (PAIR) mma_commit_pair(&acc_full[acc], 0x3);
+                else mma_commit(&acc_full[acc]);
+              }
             }
-            if (kb + n == kb1) {
-              if constexpr (PAIR) mma_commit_pair(&acc_full[acc], 0x3);
-              else mma_commit(&acc_full[acc]);
-            }
-          }
-          __syncwarp();
-          issued = true;
-        }
-      }
+            __syncwarp();
+            issued = true;
+          });
       if (stop && issued && lane == 0) {  // the products under way end before the CTA is torn down
         if constexpr (PAIR) mma_commit_pair(drain, 0x1);
         else mma_commit(drain);
