@@ -507,7 +507,8 @@ PQ8_API int pq8_layer_norm_quantize(const void* x, int type, long long ld, const
  * even: no packed layout). bias: float[n] or NULL; resid: y's type and
  * shape (EPI_RESIDUAL only), may be y itself. y may overlap none of the other inputs.
  * The last bits of a SiLU or GLU output may depend on the token next to it (two
- * share a reciprocal); everything else of a row is its own.
+ * share a reciprocal); everything else of a row is its own. SiLU and gates hold over
+ * the whole range of z (a sigmoid below 2^-126 may be 0, SiLU of minus infinity is NaN).
  * k at most 131,056, so that no sum leaves 32 bits; m and n at most 2^30. */
 PQ8_API int pq8_gemm_i8(const int8_t* w, const float* w_scale, const int8_t* x, const float* x_scale, void* y,
                         int y_type, const float* bias, const void* resid, int m, int n, int k, int epilogue,

@@ -230,7 +230,9 @@ struct UnitNorm {
       c[i] = static_cast<float>(static_cast<double>(p.b[col + i]) - rest * scale);
     }
   }
-  __device__ __forceinline__ void apply(float (&v)[E], int epi, int round_out) const {
+  // `least`: of all values before a SiLU so far; APART: with sigmoid2_apart.
+  template <bool APART = false>
+  __device__ __forceinline__ void apply(float (&v)[E], int epi, int round_out, float& least) const {
     if constexpr (E == 1) {
       v[0] = fmaf(v[0] - hi_a, a[0], c[0]);
       if (epi == PQ8_EPI_SILU) v[0] = act_f32(v[0], PQ8_EPI_SILU);
@@ -240,7 +242,10 @@ struct UnitNorm {
         const f32x2 hi = pack2(-(UNITS == kStraddle && i >= split ? hi_b : hi_a),
                                -(UNITS == kStraddle && i + 1 >= split ? hi_b : hi_a));
         f32x2 z = fma2(add2(pack2(v[i], v[i + 1]), hi), pack2(a[i], a[i + 1]), pack2(c[i], c[i + 1]));
-        if (epi == PQ8_EPI_SILU) z = mul2(z, sigmoid2(z));
+        if (epi == PQ8_EPI_SILU) {
+          if constexpr (!APART) take_least(z, least);
+          z = mul2(z, sigmoid2<APART>(z));
+        }
         unpack2(z, &v[i], &v[i + 1]);
       }
     }
@@ -277,6 +282,20 @@ __device__ __forceinline__ void store_values(T* p, const float (&v)[E]) {
       for (int j = 0; j < C; ++j) u[j] = v[i + j];
       store_chunk<T, C>(p + i, true, u);
     }
+  }
+}
+
+// Rows r0, r0 + step, ... below r1 of one unit once more, where a sigmoid was out of the fast form's range.
+template <typename T, int UNITS, typename Out>
+__device__ __forceinline__ void norm_rows_apart(const GroupNormParams& p, const UnitNorm<UNITS, kUnit<T, UNITS>>& norm,
+                                                const T* xu, Out* yu, int r0, int r1, int step, float least) {
+  if (least >= kSigmoidLeast) return;
+#pragma unroll 1
+  for (int r = r0; r < r1; r += step) {
+    float v[kUnit<T, UNITS>];
+    load_unit<T, UNITS>(xu + static_cast<size_t>(r) * p.channels, v);
+    norm.template apply<true>(v, p.epi, p.round_out, least);
+    store_values(yu + static_cast<size_t>(r) * p.channels, v);
   }
 }
 
@@ -394,18 +413,19 @@ __global__ void __launch_bounds__(kNormThreads)
       const int col = g0 * cg + u * E;
       const UnitNorm<UNITS, E> norm(p, stat, u, cg, ng, col);
       Out* const yu = y + col;
-      float v[E];
+      float v[E], least = 0.0f;
 #pragma unroll 2
       for (int r = r0 + sh.y; r < held_end; r += sh.ty) {
         load_unit<T, UNITS>(reinterpret_cast<const T*>(held + static_cast<size_t>(r - r0) * sh.units + u), v);
-        norm.apply(v, p.epi, p.round_out);
+        norm.apply(v, p.epi, p.round_out, least);
         store_values(yu + static_cast<size_t>(r) * p.channels, v);
       }
       for (int r = held_end + sh.y; r < r1; r += sh.ty) {
         load_unit<T, UNITS>(x + static_cast<size_t>(r) * p.channels + u * E, v);
-        norm.apply(v, p.epi, p.round_out);
+        norm.apply(v, p.epi, p.round_out, least);
         store_values(yu + static_cast<size_t>(r) * p.channels, v);
       }
+      norm_rows_apart<T, UNITS>(p, norm, x + u * E, yu, r0 + sh.y, r1, sh.ty, least);
     }
   }
   if (parts > 1) {
@@ -554,6 +574,7 @@ __global__ void __launch_bounds__(kNormThreads)
         T* const yu = y + col;
         constexpr int kAhead = 4;
         int r = r0 + sh.y;
+        float least = 0.0f;
         for (; r + (kAhead - 1) * sh.ty < r1; r += kAhead * sh.ty) {
           float v[kAhead][E];
 #pragma unroll
@@ -561,16 +582,17 @@ __global__ void __launch_bounds__(kNormThreads)
             load_unit<T, UNITS>(xu + static_cast<size_t>(r + k * sh.ty) * p.channels, v[k]);
 #pragma unroll
           for (int k = 0; k < kAhead; ++k) {
-            norm.apply(v[k], p.epi, p.round_out);
+            norm.apply(v[k], p.epi, p.round_out, least);
             store_values(yu + static_cast<size_t>(r + k * sh.ty) * p.channels, v[k]);
           }
         }
         for (; r < r1; r += sh.ty) {
           float v[E];
           load_unit<T, UNITS>(xu + static_cast<size_t>(r) * p.channels, v);
-          norm.apply(v, p.epi, p.round_out);
+          norm.apply(v, p.epi, p.round_out, least);
           store_values(yu + static_cast<size_t>(r) * p.channels, v);
         }
+        norm_rows_apart<T, UNITS>(p, norm, xu, yu, r0 + sh.y, r1, sh.ty, least);
       }
     }
   });

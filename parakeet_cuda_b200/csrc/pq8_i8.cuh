@@ -325,10 +325,11 @@ __device__ __forceinline__ void i8_epilogue(int epi, F&& f) {
 // nothing) from their sums v, token scales sx, channel scale t and bias b;
 // `cols` elements apart at y. Every lane of the warp takes part. GLU: lanes
 // 0-15 have a value channel and lanes 16-31 its gate; of each two tokens
-// the lower lane finishes the first and the upper lane the second.
-template <typename T, int E, int EPI>
+// the lower lane finishes the first and the upper lane the second. least: of the values before
+// a sigmoid so far. APART: with sigmoid2_apart.
+template <typename T, int E, int EPI, bool APART = false>
 __device__ __forceinline__ void i8_finish(const uint32_t (&v)[E], const T (&rv)[E], const float* sx, float t, float b,
-                                          float alpha, T* y, int cols, int cnt) {
+                                          float alpha, T* y, int cols, int cnt, float& least) {
   constexpr bool kGlu = EPI == PQ8_EPI_GLU;
   constexpr int N = kGlu ? E / 2 : E;  // outputs of this lane
   const bool upper = (threadIdx.x & 16) != 0;
@@ -348,13 +349,15 @@ __device__ __forceinline__ void i8_finish(const uint32_t (&v)[E], const T (&rv)[
         a_prev = a;
         g_prev = gate;
       } else {
-        unpack2(mul2(pack2(a_prev, a), sigmoid2(pack2(g_prev, gate))), &out[j / 2 - 1], &out[j / 2]);
-        if (g_prev != g_prev) out[j / 2 - 1] = g_prev;  // sigmoid2 caps a NaN
-        if (gate != gate) out[j / 2] = gate;
+        take_least(pack2(g_prev, gate), least);
+        unpack2(mul2(pack2(a_prev, a), sigmoid2<APART>(pack2(g_prev, gate))), &out[j / 2 - 1], &out[j / 2]);
       }
     } else {
       if constexpr (EPI == PQ8_EPI_RESIDUAL) z = fma2(pack2(alpha, alpha), z, pack2(to_f32(rv[j]), to_f32(rv[j + 1])));
-      if constexpr (EPI == PQ8_EPI_SILU) z = mul2(z, sigmoid2(z));
+      if constexpr (EPI == PQ8_EPI_SILU) {
+        take_least(z, least);
+        z = mul2(z, sigmoid2<APART>(z));
+      }
       unpack2(z, &out[j], &out[j + 1]);
       if constexpr (EPI == PQ8_EPI_RELU) {
         out[j] = relu_f32(out[j]);
@@ -373,6 +376,13 @@ __device__ __forceinline__ void i8_finish(const uint32_t (&v)[E], const T (&rv)[
     for (int j = 0; j < N; ++j)
       if (j * kStep < mine) y0[static_cast<size_t>(j * kStep) * cols] = from_f32<T>(out[j]);
   }
+}
+
+// Residuals of `cnt` <= E tokens from m0 on of one channel.
+template <typename T, int E>
+__device__ __forceinline__ void i8_load_resid(T (&rv)[E], const T* res, int m0, int cols, int cnt) {
+#pragma unroll
+  for (int j = 0; j < E; ++j) rv[j] = j < cnt ? res[static_cast<size_t>(m0 + j) * cols] : from_f32<T>(0.0f);
 }
 
 template <typename T, int BN, bool PAIR>
@@ -578,19 +588,6 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR>::kThreads, 1)
       const T* const res = static_cast<const T*>(p.resid) + col;
       const int cols = p.out_cols;
 
-      // outputs of `cnt` tokens from m0 on, whose sums are v[0 .. cnt)
-      auto finish = [&](const uint32_t(&v)[E], const T(&rv)[E], const float* sx, int m0, int cnt) {
-        T* const yp = y + static_cast<size_t>(m0) * cols;
-        i8_epilogue(p.epi, [&](auto epi) {
-          i8_finish<T, E, decltype(epi)::value>(v, rv, sx, t, b, p.alpha, yp, cols, valid ? cnt : 0);
-        });
-      };
-      auto load_resid = [&](T(&rv)[E], int m0, int cnt) {
-        if (p.epi == PQ8_EPI_RESIDUAL) {
-#pragma unroll
-          for (int j = 0; j < E; ++j) rv[j] = (valid && j < cnt) ? res[static_cast<size_t>(m0 + j) * cols] : from_f32<T>(0.0f);
-        }
-      };
       // the scales of up to kCols tokens from m0 on, for this warp
       auto load_scales = [&](int m0) {
         __syncwarp();  // the previous tile's have been read
@@ -599,32 +596,60 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR>::kThreads, 1)
           if (i + lane < C::kCols) sx[i + lane] = m0 + i + lane < p.m ? __ldg(p.x_scale + m0 + i + lane) : 0.0f;
         __syncwarp();
       };
-      T rv[E];
       if (!split) {
         const int first = token0 + group * C::kCols;
         load_scales(first);
-        load_resid(rv, first, min(E, p.m - first));
-        if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag, status)) break;
-        tc_fence_after();
-#pragma unroll 1
-        for (int cc = 0; cc < C::kChunks; ++cc) {
-          const int m0 = first + cc * E, cnt = min(E, p.m - m0);
-          uint32_t v[E];
-          tmem_ld_cols<E>(tmem + lane_base + acc * BN + group * C::kCols + cc * E, v);
-          tmem_wait_ld();
-          if (cc + 1 == C::kChunks) {
+        bool ok = true;
+        // (One kind per loop: 16 registers of residuals are held where there are any.)
+        i8_epilogue(p.epi, [&](auto epi) {
+          constexpr int EPI = decltype(epi)::value;
+          constexpr bool kSigmoid = EPI == PQ8_EPI_SILU || EPI == PQ8_EPI_GLU;
+          auto release = [&] {  // every lane has read its sums: the accumulator is free
             tc_fence_before();
-            __syncwarp();  // every lane has read its sums: the accumulator is free
+            __syncwarp();
             if (lane == 0) {
               if (PAIR) mbar_arrive_cluster(acc_empty_at + acc * 8);
               else mbar_arrive(&acc_empty[acc]);
             }
+          };
+          T rv[E];
+          if constexpr (EPI == PQ8_EPI_RESIDUAL) i8_load_resid<T, E>(rv, res, first, cols, valid ? min(E, p.m - first) : 0);
+          ok = mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag, status);
+          if (!ok) return;
+          tc_fence_after();
+          float least = 0.0f;
+#pragma unroll 1
+          for (int cc = 0; cc < C::kChunks; ++cc) {
+            const int m0 = first + cc * E, cnt = min(E, p.m - m0);
+            uint32_t v[E];
+            tmem_ld_cols<E>(tmem + lane_base + acc * BN + group * C::kCols + cc * E, v);
+            tmem_wait_ld();
+            if (!kSigmoid && cc + 1 == C::kChunks) release();
+            if (cnt > 0) {
+              T* const yp = y + static_cast<size_t>(m0) * cols;
+              i8_finish<T, E, EPI>(v, rv, sx + cc * E, t, b, p.alpha, yp, cols, valid ? cnt : 0, least);
+              if constexpr (EPI == PQ8_EPI_RESIDUAL)
+                if (cc + 1 < C::kChunks) i8_load_resid<T, E>(rv, res, m0 + E, cols, valid ? min(E, p.m - m0 - E) : 0);
+            }
           }
-          if (cnt > 0) {
-            finish(v, rv, sx + cc * E, m0, cnt);
-            if (cc + 1 < C::kChunks) load_resid(rv, m0 + E, min(E, p.m - m0 - E));
+          if constexpr (kSigmoid) {
+            // a sigmoid below the fast form's range: the warp's part once more, so that the sums
+            // have to stay until here
+            if (__any_sync(0xffffffffu, !(least >= kSigmoidLeast))) {
+#pragma unroll 1
+              for (int cc = 0; cc < C::kChunks && first + cc * E < p.m; ++cc) {
+                const int m0 = first + cc * E;
+                uint32_t v[E];
+                tmem_ld_cols<E>(tmem + lane_base + acc * BN + group * C::kCols + cc * E, v);
+                tmem_wait_ld();
+                i8_finish<T, E, EPI, true>(v, rv, sx + cc * E, t, b, p.alpha, y + static_cast<size_t>(m0) * cols, cols,
+                                           valid ? min(E, p.m - m0) : 0, least);
+              }
+            }
+            release();
           }
-        }
+        });
+        if (!ok) break;
       } else {
         // K split: this CTA's sums to shared memory, [token][channel] (the
         // ring: every load has been multiplied) ...
@@ -661,11 +686,20 @@ __global__ void __launch_bounds__(I8Cfg<BN, PAIR>::kThreads, 1)
 #pragma unroll 1
         for (int c0 = 0; c0 < cnt_all; c0 += E) {
           const int cnt = min(E, cnt_all - c0), m0 = token0 + off + c0;
-          load_resid(rv, m0, cnt);
-          uint32_t v[E];
+          i8_epilogue(p.epi, [&](auto epi) {
+            constexpr int EPI = decltype(epi)::value;
+            T rv[E];
+            if constexpr (EPI == PQ8_EPI_RESIDUAL) i8_load_resid<T, E>(rv, res, m0, cols, valid ? cnt : 0);
+            uint32_t v[E];
 #pragma unroll
-          for (int j = 0; j < E; ++j) v[j] = j < cnt ? static_cast<uint32_t>(stage[(off + c0 + j) * 128 + r]) : 0u;
-          finish(v, rv, sx + c0, m0, cnt);
+            for (int j = 0; j < E; ++j) v[j] = j < cnt ? static_cast<uint32_t>(stage[(off + c0 + j) * 128 + r]) : 0u;
+            T* const yp = y + static_cast<size_t>(m0) * cols;
+            float least = 0.0f;
+            i8_finish<T, E, EPI>(v, rv, sx + c0, t, b, p.alpha, yp, cols, valid ? cnt : 0, least);
+            if constexpr (EPI == PQ8_EPI_SILU || EPI == PQ8_EPI_GLU)
+              if (__any_sync(0xffffffffu, !(least >= kSigmoidLeast)))
+                i8_finish<T, E, EPI, true>(v, rv, sx + c0, t, b, p.alpha, yp, cols, valid ? cnt : 0, least);
+          });
         }
       }
     }
