@@ -60,7 +60,7 @@ ELEMENT_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat1
 
 class _Int8Rows:
     """A dense int8 matrix with a float32 scale per row, checked once when it is made."""
-    __slots__ = ('_q', '_scale', 'n', 'k', 'device')
+    __slots__ = ('_q', '_scale', 'n', 'k', 'device', '_at')
     q = property(lambda self: self._q)
     scale = property(lambda self: self._scale)
 
@@ -72,16 +72,18 @@ class _Int8Rows:
         self.n, self.k = q.shape
         if scale.shape[0] != self.n:
             raise ValueError(f'{self.n} rows need {self.n} scales, got {scale.shape[0]}')
-        self.device = q.device
-        if scale.device != self.device:
+        self._at = q.get_device()
+        if scale.get_device() != self._at:
             raise ValueError(f'q is on {q.device}, scale on {scale.device}')
-        self._q, self._scale = q, scale
+        self._q, self._scale, self.device = q, scale, q.device
 
     def pointers(self) -> tuple[int, int]:
         """Addresses of the integers and the scales, as they are now (a tensor can be given other memory)."""
         q, scale = self._q, self._scale
-        if q.nbytes != self.n * self.k or scale.nbytes != 4 * self.n or not (q.is_contiguous() and scale.is_contiguous()):
-            raise ValueError('the integers or the scales have changed their shape or type')
+        if (q.nbytes != self.n * self.k or scale.nbytes != 4 * self.n or q.dtype is not torch.int8
+                or scale.dtype is not torch.float32 or q.get_device() != self._at or scale.get_device() != self._at
+                or not (q.is_contiguous() and scale.is_contiguous())):
+            raise ValueError('the integers or the scales have changed their size, type, layout or device')
         return q.data_ptr(), scale.data_ptr()
 
 
@@ -326,7 +328,7 @@ class Runtime:
     # allocated by the cheapest call torch has for it.
     def _check(self, t: torch.Tensor, what: str, dtype, shape) -> int:
         """Address of a dense tensor of ``dtype`` and ``shape`` on this device."""
-        if t.dtype != dtype or t.shape != shape or t.device != self.device or not t.is_contiguous():
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self.device.index or not t.is_contiguous():
             raise ValueError(f'{what} must be contiguous {dtype} {tuple(shape)} on {self.device}, got '
                              f'{"" if t.is_contiguous() else "strided "}{t.dtype} {tuple(t.shape)} on {t.device}')
         return t.data_ptr()
@@ -334,7 +336,7 @@ class Runtime:
     def _check_rows(self, x: torch.Tensor) -> tuple[int, int, int, int]:
         """(rows, width, row distance, type code) of a matrix whose rows are dense."""
         kind = ELEMENT_TYPES.get(x.dtype)
-        if kind is None or x.dim() != 2 or x.device != self.device:
+        if kind is None or x.dim() != 2 or x.get_device() != self.device.index:
             raise ValueError(f'x must be a float32, float16 or bfloat16 matrix on {self.device}, got {x.dtype} '
                              f'{tuple(x.shape)} on {x.device}')
         rows, width = x.shape
@@ -396,7 +398,7 @@ class Runtime:
         plain rows of ``w`` (gates in the second half). ``out_dtype``: float32 (the default),
         float16 or bfloat16; ``out``, ``resid`` have it. ``out`` may be ``resid``, no other input."""
         device = self.device
-        if type(w) is not Int8Weight or w.device != device:
+        if type(w) is not Int8Weight or w._at != device.index:
             raise ValueError(f'the weight must be an Int8Weight on {device}')
         n, k = w.n, w.k
         quantized = type(x) is QuantizedRows
@@ -404,7 +406,7 @@ class Runtime:
             rows, width = x.n, x.k
             if norm is not None:
                 raise ValueError('quantised tokens take no norm')
-            if x.device != device:
+            if x._at != device.index:
                 raise ValueError(f'x is on {x.device}, the runtime on {device}')
         else:
             rows, width, ld, kind = self._check_rows(x)

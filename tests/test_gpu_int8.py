@@ -492,3 +492,22 @@ def test_past_32_bit_offsets(rt):
     near = rt.quantize_rows(x[:9, :64].contiguous())
     got = rt.quantize_rows(far)
     assert torch.equal(got.q, near.q) and torch.equal(got.scale, near.scale)
+
+
+def test_int8_rows_whose_memory_leaves_the_device(rt):
+    """Weights and tokens whose tensors were moved to the host after they were made are refused, not read."""
+    x = torch.ones(9, 64, device='cuda')
+    for part in ('q', 'scale'):
+        w8 = Int8Weight(torch.ones(32, 64, dtype=torch.int8, device='cuda'), torch.ones(32, device='cuda'))
+        rows = rt.quantize_rows(x)
+        want = rt.linear_i8(rows, w8)
+        for held in (w8, rows):
+            t = getattr(held, part)
+            kept = t.data
+            t.data = t.cpu()
+            with pytest.raises(ValueError):
+                rt.linear_i8(rows, w8)
+            t.data = kept
+        assert torch.equal(rt.linear_i8(rows, w8), want)
+    with pytest.raises(ValueError):
+        rt.linear_i8(x.cpu(), w8)

@@ -182,3 +182,19 @@ def test_group_norm_workspace_sizes(lib):
                 need = lib.group_norm_workspace_size(2, rows_, windows, c, g, ragged, quantize)
                 assert 0 <= need < 1 << 48, (rows_, windows, c, g)
                 assert need or not quantize
+
+
+def test_int8_rows_whose_memory_is_of_another_type():
+    """Integers or scales whose tensors were given memory of the same size but another type are refused."""
+    import torch
+    from parakeet_cuda_b200.runtime import Int8Weight
+    q, s = torch.ones(32, 64, dtype=torch.int8), torch.ones(32)
+    w8 = Int8Weight(q, s)
+    assert w8.pointers() == (q.data_ptr(), s.data_ptr())
+    for t, other in ((q, torch.ones(32, 16)), (s, torch.ones(32, dtype=torch.int32))):
+        kept = t.data
+        t.data = other
+        with pytest.raises(ValueError):
+            w8.pointers()
+        t.data = kept
+    assert w8.pointers() == (q.data_ptr(), s.data_ptr())
