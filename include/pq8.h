@@ -553,7 +553,9 @@ PQ8_API int pq8_group_norm(const void* x, int type, const float* w, const float*
                            const int* offsets, int channels, int groups, double eps, int activation, int flags,
                            void* workspace, size_t workspace_bytes, void* stream);
 /* The same, its rows quantised as pq8_quantize_rows quantises them (channels
- * a multiple of 16): q [rows][channels], scale [rows], for pq8_gemm_i8. */
+ * a multiple of 16): q [rows][channels], scale [rows], for pq8_gemm_i8. Rows in no
+ * window become zeros with scale 0, so that the product adds nothing to their
+ * residual. */
 PQ8_API int pq8_group_norm_quantize(const void* x, int type, const float* w, const float* b, int8_t* q, float* scale,
                                     int rows, int windows, const int* offsets, int channels, int groups, double eps,
                                     int activation, void* workspace, size_t workspace_bytes, void* stream);

@@ -2807,7 +2807,7 @@ extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, 
   const size_t q_bytes = static_cast<size_t>(rows) * channels, x_bytes = q_bytes * type_size(type);
   rc = check_group_norm(x, type, w, b, q, q_bytes, rows, windows, offsets, channels, groups, eps, activation,
                         workspace);
-  if (rc || rows == 0 || windows == 0) return rc;
+  if (rc || rows == 0) return rc;
   const size_t scale_bytes = static_cast<size_t>(rows) * 4, w_bytes = static_cast<size_t>(channels) * 4;
   if (scale == nullptr || overlap(scale, scale_bytes, x, x_bytes) || overlap(scale, scale_bytes, q, q_bytes) ||
       overlap(scale, scale_bytes, w, w_bytes) || overlap(scale, scale_bytes, b, w_bytes) ||
@@ -2816,6 +2816,11 @@ extern "C" int pq8_group_norm_quantize(const void* x, int type, const float* w, 
   if (!aligned(q, 16) || !aligned(scale, 4)) return PQ8_ERR_MISALIGNED;
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
+  if (windows == 0) {  // every row is in no window
+    if (q == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+    const cudaError_t err = cudaMemsetAsync(q, 0, q_bytes, static_cast<cudaStream_t>(stream));
+    return to_code(err != cudaSuccess ? err : cudaMemsetAsync(scale, 0, scale_bytes, static_cast<cudaStream_t>(stream)));
+  }
   const bool vec = aligned(x, 16) && aligned(w, 16) && aligned(b, 16);
   const GroupNormPlan g =
       plan_group_norm(type_size(type), vec, rows, windows, offsets != nullptr, channels, groups, true);

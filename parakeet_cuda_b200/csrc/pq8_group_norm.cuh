@@ -598,6 +598,15 @@ __global__ void __launch_bounds__(kNormThreads)
   });
 }
 
+// A row of no window, for a team of THREADS threads: integers and scale 0, so
+// that a product that follows adds nothing there.
+template <int THREADS>
+__device__ __forceinline__ void zero_row(const GroupNormParams& p, int row, int8_t* q, float* scale, int index) {
+  uint4* const at = reinterpret_cast<uint4*>(q + static_cast<size_t>(row) * p.channels);
+  for (int c = index; c < p.channels / 16; c += THREADS) at[c] = make_uint4(0, 0, 0, 0);
+  if (index == 0) scale[row] = 0.0f;
+}
+
 // Normalise, activate and quantise one block of rows: rows whole, as their
 // scale needs every channel.
 template <typename T, int CHUNKS, int WARPS, bool VEC>
@@ -630,7 +639,15 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       for (int c = (threadIdx.x & 31) * 128 / static_cast<int>(sizeof(T)); c < p.channels; c += 32 * 128 / static_cast<int>(sizeof(T)))
         asm volatile("prefetch.global.L1 [%0];" ::"l"(x + c));
   }
+  const int my_team = static_cast<int>(threadIdx.x) / (32 * WARPS);
+  int done = b0;  // the block's rows that are written, or in a window
+  auto zero_up_to = [&](int end) {
+    for (int r = done + my_team; r < end; r += kTeams) zero_row<32 * WARPS>(p, r, q, scale, team.index());
+    done = max(done, end);
+  };
   block_windows(p, b0, b1, [&](int w, int lo, int hi, int r0, int r1) {
+    zero_up_to(r0);
+    done = max(done, r1);
     group_finish<T>(p, partial, w, lo, hi, 0, p.groups, stat);
     for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
       const float m = static_cast<float>(stat[g].mean);
@@ -638,12 +655,13 @@ __global__ void __launch_bounds__(kRowThreads, 2)
                             static_cast<float>(stat[g].rstd), 0.0f);
     }
     __syncthreads();
-    for (int r = r0 + static_cast<int>(threadIdx.x) / (32 * WARPS); r < r1; r += kTeams) {
+    for (int r = r0 + my_team; r < r1; r += kTeams) {
       src.x = static_cast<const T*>(p.x) + static_cast<size_t>(r) * p.channels;
       const float s = quantize_row<CHUNKS, WARPS, false>(src, p.channels, q + static_cast<size_t>(r) * p.channels, team);
       if (team.index() == 0) scale[r] = s;
     }
   });
+  zero_up_to(b1);
 }
 
 // The second half of the quantised form where the first was one launch: rows of
@@ -702,7 +720,10 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   const int first = static_cast<int>(blockIdx.x) * kTeams + static_cast<int>(threadIdx.x) / (32 * WARPS);
   for (int row = first; row < p.rows; row += static_cast<int>(gridDim.x) * kTeams) {
     const int w = row_window(p, row);
-    if (w < 0) continue;  // the whole team
+    if (w < 0) {  // the whole team
+      zero_row<32 * WARPS>(p, row, q, scale, team.index());
+      continue;
+    }
     const size_t at = static_cast<size_t>(row) * p.channels;
     src.y = y + at;
     src.x = static_cast<const T*>(p.x) + at;

@@ -480,7 +480,7 @@ class Runtime:
     def group_norm_quantize(self, x: torch.Tensor, weight, bias, groups: int, windows: int = 1, offsets=None,
                             eps: float = 1e-5, epilogue: int = EPI_NONE) -> QuantizedRows:
         """``group_norm``, its rows quantised as ``quantize_rows`` does, for ``linear_i8``. Rows in no window
-        have no values and no scale."""
+        are zeros with scale 0: a ``linear_i8`` that follows leaves their residual as it is."""
         rows, channels, kind, at, off = self._check_group_norm(x, weight, bias, groups, windows, offsets)
         out = QuantizedRows(torch.empty(rows, channels, dtype=torch.int8, device=self.device),
                             torch.empty(rows, dtype=torch.float32, device=self.device))

@@ -1,0 +1,92 @@
+"""Windows of the quantised group norm that leave rows out, and many windows. The oracle and the
+tolerances are those of test_gpu_group_norm.py: integers equal but for values within 1e-9 of a border, scales
+within one step of fp32."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import int8 as oi
+from parakeet_cuda_b200.pq8 import EPI_RESIDUAL, EPI_SILU
+from parakeet_cuda_b200.runtime import ELEMENT_TYPES, Int8Weight, Runtime
+
+pytestmark = pytest.mark.gpu
+
+TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+@pytest.fixture(scope='module')
+def rt():
+    return Runtime(0)
+
+
+def dev(a, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return t if dtype is None else t.to(dtype)
+
+
+def f64(t):
+    return t.double().cpu().numpy()
+
+
+def inputs(seed, rows, channels, dtype, skip=0):
+    rng = np.random.default_rng(seed)
+    flat = dev(rng.normal(size=rows * channels + skip).astype(np.float32) + 0.5, dtype)
+    w, b = 1 + 0.2 * rng.normal(size=channels), 0.2 * rng.normal(size=channels)
+    return flat[skip:].view(rows, channels), dev(w.astype(np.float32)), dev(b.astype(np.float32))
+
+
+def check_quantized(q, scale, x, w, b, groups, bounds, act):
+    h = oi.group_norm(f64(x), f64(w), f64(b), groups, bounds, epilogue=act)
+    inside = np.zeros(len(h), bool)
+    for lo, hi in zip(bounds[:-1], bounds[1:]):
+        inside[lo:hi] = True
+    wq, ws, margin = oi.quantize(h[inside])
+    q, scale = q.cpu().numpy(), scale.cpu().numpy()
+    assert (np.abs(scale[inside] - ws) <= 2.0 ** -23 * ws).all()
+    wrong = q[inside] != wq
+    assert not (wrong & (margin > 1e-9) & (scale[inside] == ws)[:, None]).any(), int(wrong.sum())
+    assert not q[~inside].any() and (scale[~inside] == 0).all()
+
+
+# rows left out before, behind and (by offsets that start past 0) around one window; empty windows at both ends; none
+BOUNDS = [[0, 0, 0, 7, 90, 90, 200, 200], [13, 20, 64, 187], [60, 140], [100, 100], [200, 200, 200], [0]]
+
+
+@pytest.mark.parametrize('bounds', BOUNDS)
+@pytest.mark.parametrize('channels,groups,skip', [(64, 4, 0), (1024, 32, 0), (1040, 8, 0), (64, 4, 1), (9008, 1, 0)])
+def test_quantize_leaves_rows_out(rt, bounds, channels, groups, skip):
+    """Rows of no window are zeros with scale 0, whatever the buffers held, in every kernel form."""
+    rows, windows = 200, len(bounds) - 1
+    off = torch.tensor(bounds, dtype=torch.int32, device='cuda')
+    for dtype in TYPES:
+        x, w, b = inputs(channels + windows, rows, channels, dtype, skip)
+        q = torch.full((rows + 2, channels), 77, dtype=torch.int8, device='cuda')
+        scale = torch.full((rows + 2,), float('nan'), device='cuda')
+        kind = ELEMENT_TYPES[dtype]
+        need = rt.lib.group_norm_workspace_size(kind, rows, windows, channels, groups, True, True, skip == 0)
+        ws = torch.empty(need, dtype=torch.uint8, device='cuda')
+        rt.lib.call('pq8_group_norm_quantize', x.data_ptr(), kind, w.data_ptr(), b.data_ptr(), q[1:].data_ptr(),
+                    scale[1:].data_ptr(), rows, windows, off.data_ptr(), channels, groups, 1e-5, EPI_SILU, ws.data_ptr(), need,
+                    rt.stream())
+        check_quantized(q[1:rows + 1], scale[1:rows + 1], x, w, b, groups, bounds, 'silu')
+        assert (q[0] == 77).all() and (q[-1] == 77).all() and torch.isnan(scale[[0, rows + 1]]).all()
+
+
+def test_conv_module_tail_keeps_other_rows(rt):
+    """Rows of no window keep the residual stream they had, bit for bit, in place too."""
+    rng = np.random.default_rng(3)
+    for bounds in ([30, 40, 40, 155, 230], [100, 101], [0]):
+        windows = len(bounds) - 1
+        off = torch.tensor(bounds, dtype=torch.int32, device='cuda')
+        x, w, b = inputs(4, 260, 1024, torch.float32)
+        w8 = Int8Weight(dev(rng.integers(-127, 128, size=(1024, 1024)).astype(np.int8)), dev(rng.uniform(1e-3, 2e-3, 1024).astype(np.float32)))
+        resid = dev(rng.normal(size=(260, 1024)).astype(np.float32))
+        torch.full((64, 1 << 20), float('nan'), device='cuda')  # what a new tensor may find in its memory
+        h = rt.group_norm_quantize(x, w, b, 32, windows=windows, offsets=off, epilogue=EPI_SILU)
+        want = rt.linear_i8(h, w8, resid=resid, epilogue=EPI_RESIDUAL)
+        for outside in (slice(0, bounds[0]), slice(bounds[-1], 260)):
+            assert torch.equal(want[outside], resid[outside])
+        stream = resid.clone()
+        rt.linear_i8(h, w8, out=stream, resid=stream, epilogue=EPI_RESIDUAL)
+        assert torch.equal(stream, want)
+        assert not torch.equal(want[bounds[0]:bounds[-1]], resid[bounds[0]:bounds[-1]]) or bounds[0] == bounds[-1]
