@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kNormThreads)
   const bool active = sh.y < sh.ty;
   // A thread reads back only what it has put there itself, so no barrier. Its
   // rows arrive in four groups; the sums of one are taken while the next are
-  // under way. (Several units per thread: a slab of one wide group.)
+  // under way.
   const int mine = active && held_end > r0 + sh.y ? (held_end - r0 - sh.y + sh.ty - 1) / sh.ty : 0;
   const int quarter = (mine + 3) / 4;
 #pragma unroll
@@ -358,29 +358,39 @@ __global__ void __launch_bounds__(kNormThreads)
   unit_group<UNITS, E>(min(sh.x, sh.units - 1), cg, &g, &split);  // the same for all of a thread's units
   UnitSum<UNITS, E, QUANT> sum(split, first_value<T>(p, lo, hi, g0, g, cg),
                                UNITS == kStraddle && split < E ? first_value<T>(p, lo, hi, g0, g + 1, cg) : 0.0);
+  if (sh.units <= sh.tx) {  // one unit per thread
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (k == 0) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else if (k == 1) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (k == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    for (int k = 0; k < 4; ++k) {
+      if (k == 0) asm volatile("cp.async.wait_group 3;" ::: "memory");
+      else if (k == 1) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else if (k == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll 2
-    for (int i = k * quarter; i < min(mine, (k + 1) * quarter); ++i) {
-      const int r = sh.y + i * sh.ty;
-      for (int u = sh.x; u < sh.units; u += sh.tx) {
+      for (int i = k * quarter; i < min(mine, (k + 1) * quarter); ++i) {
         float v[E];
-        load_unit<T, UNITS>(reinterpret_cast<const T*>(held + static_cast<size_t>(r) * sh.units + u), v);
+        load_unit<T, UNITS>(reinterpret_cast<const T*>(held + static_cast<size_t>(sh.y + i * sh.ty) * sh.units + sh.x), v);
         sum.add(acc, v);
       }
     }
-  }
-  if (active) {
-    for (int r = held_end + sh.y; r < r1; r += sh.ty)
-      for (int u = sh.x; u < sh.units; u += sh.tx) {
+    if (active)
+      for (int r = held_end + sh.y; r < r1; r += sh.ty) {
         float v[E];
-        load_unit<T, UNITS>(x + static_cast<size_t>(r) * p.channels + u * E, v);
+        load_unit<T, UNITS>(x + static_cast<size_t>(r) * p.channels + sh.x * E, v);
         sum.add(acc, v);
       }
+  } else {  // a group wider than the CTA: unit by unit, so that a run has the rows of one column
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll 1
+    for (int u = sh.x; u < sh.units; u += sh.tx) {
+      sum.flush(acc);
+#pragma unroll 1
+      for (int r = r0 + sh.y; r < r1; r += sh.ty) {
+        float v[E];
+        load_unit<T, UNITS>(r < held_end ? reinterpret_cast<const T*>(held + static_cast<size_t>(r - r0) * sh.units + u)
+                                         : x + static_cast<size_t>(r) * p.channels + u * E, v);
+        sum.add(acc, v);
+      }
+    }
   }
   sum.flush(acc);
   reduce_groups<UNITS, E>(sh, acc, cg, ng, red, sums);

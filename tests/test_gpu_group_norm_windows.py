@@ -1,6 +1,6 @@
-"""Windows of the quantised group norm that leave rows out, and many windows. The oracle and the
-tolerances are those of test_gpu_group_norm.py: integers equal but for values within 1e-9 of a border, scales
-within one step of fp32."""
+"""The group norm's windows and groups at their edges: windows that leave rows out, groups wider than a
+CTA. The oracle and the tolerances of the quantised form are those of test_gpu_group_norm.py: integers equal but for
+values within 1e-9 of a border, scales within one step of fp32."""
 import numpy as np
 import pytest
 import torch
@@ -90,3 +90,22 @@ def test_conv_module_tail_keeps_other_rows(rt):
         rt.linear_i8(h, w8, out=stream, resid=stream, epilogue=EPI_RESIDUAL)
         assert torch.equal(stream, want)
         assert not torch.equal(want[bounds[0]:bounds[-1]], resid[bounds[0]:bounds[-1]]) or bounds[0] == bounds[-1]
+
+
+@pytest.mark.parametrize('rows,ragged', [(96, False), (96, True), (40, False), (3000, False)])
+@pytest.mark.parametrize('channels', [4096, 16384])
+def test_wide_groups_sum_by_column(rt, rows, channels, ragged):
+    """One group of more columns than a CTA has threads for. Every column has one value in all rows, so its differences
+    from its first row are 0, the sums are exact, and what is left are the roundings of the normalisation: x minus the mean,
+    the scale and the multiply-add, one each, under 4 U |z| with the mean's remainder, U for that remainder's own. (Runs that mix these
+    columns round the variance off by 28 U and the mean by 6 U deviations.)"""
+    U = 2.0 ** -24
+    value = np.array([-2.3483655, -0.90141344, -0.94846755, -1.0168121], np.float32)
+    x = np.broadcast_to(np.resize(np.repeat(value, 1024), channels), (rows, channels))
+    bounds = [3, rows - 5] if ragged else [0, rows]
+    off = torch.tensor(bounds, dtype=torch.int32, device='cuda') if ragged else None
+    w, b = torch.ones(channels, device='cuda'), torch.zeros(channels, device='cuda')
+    got = f64(rt.group_norm(dev(x), w, b, 1, offsets=off))
+    z = oi.group_norm(x, np.ones(channels), np.zeros(channels), 1, bounds)
+    inside = slice(bounds[0], bounds[-1])
+    assert (np.abs(got - z)[inside] <= U * (4 * np.abs(z) + 1)[inside]).all(), float(np.abs(got - z)[inside].max() / U)
