@@ -450,28 +450,39 @@ __global__ void __launch_bounds__(kNormThreads)
 // window by window. The sums of block b and window w go to partial[b + w]
 // (blocks and windows both follow the rows, so no two pairs meet there).
 
+// The first window from w on that ends after row r, or p.windows: a search in which
+// every thread of the CTA looks at one window (up to 256 windows in one step, 2^24 in
+// three). Every thread takes part.
+__device__ __forceinline__ int window_after(const GroupNormParams& p, int w, int r) {
+  int n = p.windows - w;  // it is one of [w, w + n]
+  while (n > 0) {
+    const int step = (n + kNormThreads - 1) / kNormThreads;
+    const int i = w + (static_cast<int>(threadIdx.x) + 1) * step - 1;
+    const int before = step * __syncthreads_count(i < w + n && p.offsets[i + 1] <= r);
+    w += before;
+    n = min(step - 1, n - before);
+  }
+  return w;
+}
+
 // f(window, its rows [lo, hi), those within [b0, b1)) for the windows with
-// rows in [b0, b1). Every thread of the CTA takes part.
+// rows in [b0, b1). Every thread of the CTA takes part. Windows of no rows are passed over by
+// search, as there may be millions of them.
 template <typename F>
 __device__ __forceinline__ void block_windows(const GroupNormParams& p, int b0, int b1, F&& f) {
-  int w = 0;
-  if (p.offsets == nullptr) {
-    w = b0 / (p.rows / p.windows);
-  } else {
-    // the windows that end at or before b0 come first
-    for (int i0 = 0; i0 < p.windows; i0 += blockDim.x) {
-      const int i = i0 + static_cast<int>(threadIdx.x);
-      const int n = __syncthreads_count(i < p.windows && p.offsets[i + 1] <= b0);
-      w += n;
-      if (n < static_cast<int>(blockDim.x)) break;
-    }
-  }
-  for (; w < p.windows; ++w) {
+  static_assert(kNormThreads == kRowThreads, "both kinds of kernel search with all their threads");
+  int w = p.offsets == nullptr ? b0 / (p.rows / p.windows) : 0;
+  bool search = p.offsets != nullptr;
+  for (int after = b0;; ++w) {
+    if (search) w = window_after(p, w, after);
+    if (w >= p.windows) break;
     int lo, hi;
     window_rows(p, w, &lo, &hi);
     if (lo >= b1) break;
     const int r0 = max(lo, b0), r1 = min(hi, b1);
-    if (r0 < r1) f(w, lo, hi, r0, r1);
+    search = r0 >= r1;
+    after = r0;
+    if (!search) f(w, lo, hi, r0, r1);
   }
 }
 

@@ -1,4 +1,4 @@
-"""The group norm's windows and groups at their edges: windows that leave rows out, groups wider than a
+"""The group norm's windows and groups at their edges: windows that leave rows out, many windows, groups wider than a
 CTA. The oracle and the tolerances of the quantised form are those of test_gpu_group_norm.py: integers equal but for
 values within 1e-9 of a border, scales within one step of fp32."""
 import numpy as np
@@ -109,3 +109,37 @@ def test_wide_groups_sum_by_column(rt, rows, channels, ragged):
     z = oi.group_norm(x, np.ones(channels), np.zeros(channels), 1, bounds)
     inside = slice(bounds[0], bounds[-1])
     assert (np.abs(got - z)[inside] <= U * (4 * np.abs(z) + 1)[inside]).all(), float(np.abs(got - z)[inside].max() / U)
+
+
+def many_windows(ends):
+    """Offsets of the windows that end at the rows ``ends``, each run of (row, how often)."""
+    return torch.tensor(np.concatenate([[0]] + [np.full(n, r) for r, n in ends]).astype(np.int32), device='cuda')
+
+
+@pytest.mark.parametrize('ends', [[(0, 300), (24, 1), (24, 300), (25, 1), (40, 700), (64, 2)],
+                                  [(i, 1) for i in range(1, 65)], [(i, 257) for i in range(1, 65)],
+                                  [(0, 1 << 21), (24, 1 << 21), (60, 1 << 20)]])
+def test_many_windows(rt, ends):
+    """Windows without rows between those with some, by the hundred and by the million. A million empty windows cost
+    no more than a few: walked one after the other they took seconds, longer than the limit (4 s) of a wait in
+    the product that follows. (The bound of 50 ms is a thousand times what the search takes.)"""
+    off = many_windows(ends)
+    rows, windows = 70, off.numel() - 1
+    bounds = [0] + [r for r, _ in ends]
+    for dtype, channels, groups, skip in ((torch.float32, 64, 4, 0), (torch.float16, 1040, 8, 0), (torch.float32, 64, 4, 1)):
+        x, w, b = inputs(7, rows, channels, dtype, skip)
+        out = torch.full_like(x, 9.0)
+        rt.group_norm(x, w, b, groups, windows=windows, offsets=off, out=out)
+        a, z = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        rt.group_norm(x, w, b, groups, windows=windows, offsets=off, out=out)
+        got = rt.group_norm_quantize(x, w, b, groups, windows=windows, offsets=off, epilogue=EPI_SILU)
+        z.record()
+        z.synchronize()
+        assert a.elapsed_time(z) < 50.0
+        want = oi.group_norm(f64(x), f64(w), f64(b), groups, bounds)[:bounds[-1]]
+        fi = torch.finfo(dtype)
+        # at most 64 rows: statistics and normalisation are off by under 64 x 2^-24 of the largest value
+        bound = (fi.eps / 2 + 2.0 ** -18) * np.abs(want).max() + fi.tiny
+        assert (np.abs(f64(out)[:bounds[-1]] - want) <= bound).all() and (out[bounds[-1]:] == 9).all()
+        check_quantized(got.q, got.scale, x, w, b, groups, bounds, 'silu')
