@@ -55,7 +55,9 @@ class EncoderBlocks:
         sequences = sequences and not self.int8
         self.rt, self.windows, self.t, self.layers = runtime, windows, t, layers
         self.rows = windows * t
-        self.attn_flags = FLAG_OUT_TF32 | (ATTN_FP32 if attention_fp32 else 0)
+        # what a TF32 product reads is rounded where it is written; 8-bit products quantise it as it is
+        self.out_flags = 0 if self.int8 else FLAG_OUT_TF32
+        self.attn_flags = self.out_flags | (ATTN_FP32 if attention_fp32 else 0)
         dev = runtime.device
         if self.int8:  # requantised with a scale per output channel
             self.linears = [{name: runtime.int8_weight((np.concatenate(
@@ -81,9 +83,10 @@ class EncoderBlocks:
         limit = int(model.metadata['asr.encoder.pos_emb_max_len'])
         if t > limit:
             raise ValueError(f'{t} frames exceed pos_emb_max_len {limit}')
-        # positional rows pe[limit - t : limit + t - 1] (encoder.py:71-73), TF32-rounded for linear_pos
+        # positional rows pe[limit - t : limit + t - 1] (encoder.py:71-73), TF32-rounded for a TF32 linear_pos
         self.pe = to_dev(np.asarray(model.array('encoder.pos_enc.pe'))[limit - t:limit + t - 1])
-        runtime.lib.call('pq8_round_tf32', self.pe.data_ptr(), self.pe.numel(), runtime.stream())
+        if not self.int8:
+            runtime.lib.call('pq8_round_tf32', self.pe.data_ptr(), self.pe.numel(), runtime.stream())
         rows = self.rows
         self.buf = {
             'x': torch.zeros(rows, D_MODEL, **f32),
@@ -182,7 +185,7 @@ class EncoderBlocks:
         b, (bw, bb, bm, bv) = self.buf, p['bn']
         self.rt.lib.call('pq8_conv_depthwise_bn_silu', b['gate'].data_ptr(), p['dw'].data_ptr(), bw.data_ptr(),
                          bb.data_ptr(), bm.data_ptr(), bv.data_ptr(), b['dw'].data_ptr(), self.windows, self.t, D_MODEL,
-                         FLAG_OUT_TF32, self.rt.stream())
+                         self.out_flags, self.rt.stream())
 
     def layer(self, l: int, final_norm: bool = True) -> None:
         """One block on the residual stream ``buf['x']`` (reference.py:33-66).
