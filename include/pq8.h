@@ -514,6 +514,12 @@ PQ8_API int pq8_gemm_i8(const int8_t* w, const float* w_scale, const int8_t* x, 
                         int y_type, const float* bias, const void* resid, int m, int n, int k, int epilogue,
                         float alpha, void* stream);
 
+/* The tile that pq8_gemm_i8 takes for a product of this size on the current
+ * device (nothing is enqueued): tokens of a tile, CTAs that share it (1 or 2), and
+ * CTAs that K is split over. tokens 0: the kernel for up to 8 tokens. For tests and
+ * profiles; results do not depend on it, but for what pq8_gemm_i8 says of SiLU and GLU. */
+PQ8_API int pq8_gemm_i8_tile(int m, int n, int k, int epilogue, int* tokens, int* ctas, int* k_splits);
+
 /* pq8_quantize_rows (norm_w, norm_b NULL) or pq8_layer_norm_quantize, then
  * pq8_gemm_i8: the linear on tokens in floating point. The
  * quantised tokens live in the workspace (16-byte aligned, no

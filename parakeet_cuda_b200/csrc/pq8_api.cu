@@ -2408,10 +2408,13 @@ I8Choice choose_i8(DeviceState* ds, int m, int n_tiles, int k_blocks) {
   return best;
 }
 
+I8Choice choose_i8(DeviceState* ds, int m, int n, int k, int epilogue) {
+  return choose_i8(ds, m, epilogue == PQ8_EPI_GLU ? (n / 2 + 63) / 64 : (n + 127) / 128, (k + 127) / 128);
+}
+
 template <typename T>
 int launch_i8_tiles(DeviceState* ds, const I8Params& p, cudaStream_t st) {
-  const int n_tiles = p.epi == PQ8_EPI_GLU ? (p.out_cols + 63) / 64 : (p.n + 127) / 128;
-  const I8Choice c = choose_i8(ds, p.m, n_tiles, (p.k + 127) / 128);
+  const I8Choice c = choose_i8(ds, p.m, p.n, p.k, p.epi);
   switch (c.shape) {
     case 0: return launch_i8_gemm<T, 16, false>(ds, p, c.splits, st);
     case 1: return launch_i8_gemm<T, 32, false>(ds, p, c.splits, st);
@@ -2498,6 +2501,21 @@ extern "C" int pq8_gemm_i8(const int8_t* w, const float* w_scale, const int8_t* 
   if ((rc = device_state(&ds))) return rc;
   return launch_i8(ds, i8_params(ds, w, w_scale, x, x_scale, y, bias, resid, m, n, k, epilogue, alpha), y_type,
                    static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int pq8_gemm_i8_tile(int m, int n, int k, int epilogue, int* tokens, int* ctas, int* k_splits) {
+  if (tokens == nullptr || ctas == nullptr || k_splits == nullptr) return PQ8_ERR_INVALID_ARGUMENT;
+  int rc = check_i8_args(nullptr, nullptr, nullptr, PQ8_TYPE_F32, nullptr, 0, n, k, epilogue);
+  if (rc) return rc;
+  if (m < 1 || m > kI8MaxRows) return PQ8_ERR_UNSUPPORTED_SHAPE;
+  DeviceState* ds;
+  if ((rc = device_state(&ds))) return rc;
+  const I8Choice c = choose_i8(ds, m, n, k, epilogue);
+  const bool few = m <= kI8GemvMaxM;
+  *tokens = few ? 0 : kI8Shapes[c.shape].tokens;
+  *ctas = few ? 1 : kI8Shapes[c.shape].ctas;
+  *k_splits = few ? 1 : c.splits;
+  return PQ8_OK;
 }
 
 extern "C" int pq8_linear_i8_workspace_size(int m, int k, size_t* bytes) {

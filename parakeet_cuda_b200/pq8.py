@@ -103,6 +103,7 @@ SIGNATURES = {
     'pq8_quantize_rows': ([_P, _I, _LL, _P, _P, _I, _I, _P], _I),
     'pq8_layer_norm_quantize': ([_P, _I, _LL, _P, _P, _P, _P, _I, _I, _P], _I),
     'pq8_gemm_i8': ([_P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _P], _I),
+    'pq8_gemm_i8_tile': ([_I, _I, _I, _I, C.POINTER(_I), C.POINTER(_I), C.POINTER(_I)], _I),
     'pq8_linear_i8_workspace_size': ([_I, _I, C.POINTER(_SZ)], _I),
     'pq8_linear_i8': ([_P, _P, _P, _I, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _P, _SZ, _P], _I),
     'pq8_group_norm_workspace_size': ([_I, _I, _I, _I, _I, _I, _I, _I, C.POINTER(_SZ)], _I),
@@ -187,6 +188,12 @@ class Library:
         out = _SZ()
         self.call('pq8_linear_workspace_size', m, n, k, C.byref(out))
         return out.value
+
+    def gemm_i8_tile(self, m: int, n: int, k: int, epilogue: int = EPI_NONE) -> tuple[int, int, int]:
+        """(tokens, CTAs, K splits) of the tile that ``pq8_gemm_i8`` takes; 0 tokens: the kernel for up to 8."""
+        out = _I(), _I(), _I()
+        self.call('pq8_gemm_i8_tile', m, n, k, epilogue, *(C.byref(v) for v in out))
+        return tuple(v.value for v in out)
 
     def linear_i8_workspace_size(self, m: int, k: int) -> int:
         out = _SZ()

@@ -198,3 +198,14 @@ def test_int8_rows_whose_memory_is_of_another_type():
             w8.pointers()
         t.data = kept
     assert w8.pointers() == (q.data_ptr(), s.data_ptr())
+
+
+def test_gemm_i8_tile_refusals(lib):
+    out = [C.byref(C.c_int()) for _ in range(3)]
+    tile = lambda m=4, n=64, k=64, epi=0, out=out: code(lib, 'pq8_gemm_i8_tile', m, n, k, epi, *out)
+    for kw in ({'m': 0}, {'m': -1}, {'m': (1 << 30) + 1}, {'n': 0}, {'k': 24}, {'k': pq8.I8_MAX_K + 16},
+               {'epi': pq8.EPI_GLU, 'n': 63}):
+        assert tile(**kw) == pq8.ERR_UNSUPPORTED_SHAPE, kw
+    assert tile(epi=5) == pq8.ERR_INVALID_ARGUMENT
+    for i in range(3):
+        assert tile(out=out[:i] + [None] + out[i + 1:]) == pq8.ERR_INVALID_ARGUMENT
