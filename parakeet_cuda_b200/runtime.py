@@ -31,6 +31,8 @@ MIB = 1 << 20
 # around it, which costs as much as a launch.
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+# The current device's index, without the initialisation that torch.cuda.current_device looks for first.
+_current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
 
 
 def _ptr(t) -> int | None:
@@ -353,7 +355,7 @@ class Runtime:
         """A library call on this device's current stream."""
         index = self.device.index
         args += (_raw_stream(index),)
-        if torch.cuda.current_device() == index:
+        if _current_device() == index:
             code = getattr(self.lib.lib, call)(*args)
         else:
             with torch.cuda.device(index):
@@ -361,19 +363,24 @@ class Runtime:
         if code:
             raise pq8.PQ8Error(call, code, self.lib.error_string(code))
 
+    def _new_rows(self, rows: int, width: int) -> tuple[QuantizedRows, int, int]:
+        """Rows to be written, and the addresses of their integers and scales."""
+        q = torch.empty(rows, width, dtype=torch.int8, device=self.device)
+        scale = torch.empty(rows, dtype=torch.float32, device=self.device)
+        return QuantizedRows(q, scale), q.data_ptr(), scale.data_ptr()
+
     def quantize_rows(self, x: torch.Tensor, norm=None) -> QuantizedRows:
         """``x`` [rows, width] (float32, float16 or bfloat16; rows dense, any row distance) to 8-bit
         integers with one scale per row, ``norm=(weight, bias)`` applying LayerNorm first. The
         integers are those of the exact quotient (ties to even); ``width`` a multiple of 16."""
         rows, width, ld, kind = self._check_rows(x)
-        out = QuantizedRows(torch.empty(rows, width, dtype=torch.int8, device=self.device),
-                            torch.empty(rows, dtype=torch.float32, device=self.device))
+        out, q, scale = self._new_rows(rows, width)
         if norm is None:
-            self._enqueue('pq8_quantize_rows', x.data_ptr(), kind, ld, *out.pointers(), rows, width)
+            self._enqueue('pq8_quantize_rows', x.data_ptr(), kind, ld, q, scale, rows, width)
         else:
             w = self._check(norm[0], 'the norm weight', torch.float32, (width,))
             b = self._check(norm[1], 'the norm bias', torch.float32, (width,))
-            self._enqueue('pq8_layer_norm_quantize', x.data_ptr(), kind, ld, w, b, *out.pointers(), rows, width)
+            self._enqueue('pq8_layer_norm_quantize', x.data_ptr(), kind, ld, w, b, q, scale, rows, width)
         return out
 
     def int8_weight(self, w) -> Int8Weight:
@@ -482,13 +489,12 @@ class Runtime:
         """``group_norm``, its rows quantised as ``quantize_rows`` does, for ``linear_i8``. Rows in no window
         are zeros with scale 0: a ``linear_i8`` that follows leaves their residual as it is."""
         rows, channels, kind, at, off = self._check_group_norm(x, weight, bias, groups, windows, offsets)
-        out = QuantizedRows(torch.empty(rows, channels, dtype=torch.int8, device=self.device),
-                            torch.empty(rows, dtype=torch.float32, device=self.device))
+        out, q, scale = self._new_rows(rows, channels)
         need = self.lib.group_norm_workspace_size(kind, rows, windows, channels, groups, off is not None, True,
                                                   not (at[0] | at[1] | at[2]) & 15)
         scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._enqueue('pq8_group_norm_quantize', at[0], kind, at[1], at[2], *out.pointers(), rows, windows,
-                      off, channels, groups, eps, epilogue, _ptr(scratch), need)
+        self._enqueue('pq8_group_norm_quantize', at[0], kind, at[1], at[2], q, scale, rows, windows, off,
+                      channels, groups, eps, epilogue, _ptr(scratch), need)
         return out
 
     def device_status(self) -> int:
