@@ -496,7 +496,7 @@ PQ8_API int pq8_quantize_rows(const void* x, int type, long long ld, int8_t* q, 
 
 /* LayerNorm (eps 1e-5, as pq8_layer_norm) and quantisation of its result in
  * one pass: no normalised row is written. w, b: float[width]. Mean and
- * variance are FP64. Values of 2^126 and beyond count as infinite. */
+ * variance are FP64. Values of 2^126 and beyond may count as infinite. */
 PQ8_API int pq8_layer_norm_quantize(const void* x, int type, long long ld, const float* w, const float* b, int8_t* q,
                                     float* scale, int rows, int width, void* stream);
 

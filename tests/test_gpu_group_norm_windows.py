@@ -143,3 +143,30 @@ def test_many_windows(rt, ends):
         bound = (fi.eps / 2 + 2.0 ** -18) * np.abs(want).max() + fi.tiny
         assert (np.abs(f64(out)[:bounds[-1]] - want) <= bound).all() and (out[bounds[-1]:] == 9).all()
         check_quantized(got.q, got.scale, x, w, b, groups, bounds, 'silu')
+
+
+@pytest.mark.parametrize('windows,t,channels,groups,ragged,skip', [
+    (1, 7, 1024, 32, False, 0), (8, 375, 1024, 32, False, 0), (3, 400, 1024, 1, False, 0), (5, 90, 1000, 8, False, 0), (2, 300, 35, 5, False, 0),
+    (2, 3000, 64, 1, False, 0), (4, 200, 1000, 8, True, 0), (4, 200, 96, 96, True, 0), (3, 60, 8192, 2, False, 0), (2, 200, 64, 4, False, 1),
+    (4, 2000, 256, 8, True, 1)])
+def test_statistics_of_whole_numbers(rt, windows, t, channels, groups, ragged, skip):
+    """Whole numbers from -8 to 24: every sum of differences and of their squares is a whole number below 2^24 and so
+    exact in fp32, in whatever order, and the statistics are right to fp64. What is left is the normalisation: x minus the
+    rounded mean, the scale and the multiply-add round once each, 3 U |z| (U = 2^-24), and what the mean's remainder
+    loses is of the order of U^2; then half a step of the type. (32 differences of up to 32: sums below 2^10, squares below 2^15.)"""
+    U = 2.0 ** -24
+    rng = np.random.default_rng(channels + t)
+    rows = windows * t
+    bounds = sorted(rng.integers(0, rows + 1, windows + 1).tolist()) if ragged else [i * t for i in range(windows + 1)]
+    off = torch.tensor(bounds, dtype=torch.int32, device='cuda') if ragged else None
+    x = rng.integers(-8, 25, size=(rows, channels))
+    z = oi.group_norm(x, np.ones(channels), np.zeros(channels), groups, bounds)[bounds[0]:bounds[-1]]
+    w, b = torch.ones(channels, device='cuda'), torch.zeros(channels, device='cuda')
+    for dtype in TYPES:
+        flat = torch.zeros(rows * channels + skip, dtype=dtype, device='cuda')
+        held = flat[skip:].view(rows, channels)
+        held.copy_(dev(x.astype(np.float32)))
+        got = f64(rt.group_norm(held, w, b, groups, windows=windows, offsets=off))[bounds[0]:bounds[-1]]
+        err = 3.1 * U * np.abs(z) + 2.0 ** -40
+        bound = err + (torch.finfo(dtype).eps / 2 * (np.abs(z) + err) if dtype != torch.float32 else 0.0)
+        assert (np.abs(got - z) <= bound).all(), (dtype, float((np.abs(got - z) / bound).max()))
