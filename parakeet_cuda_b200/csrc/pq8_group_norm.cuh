@@ -18,12 +18,13 @@
 // partial sums go through a workspace and a second launch reads x again.
 //
 // Measured (bytes of x and y over the time): 8 x 375 x 1024 fp32, 32 groups,
-// one launch 9.7 us (2.5 TB/s: one wave of CTAs that load, sum, meet and store in
-// turn, 14,000 cycles), 64 windows 46.5 us (4.2 TB/s); 64 x 375 x 1024 bf16 in one
-// group 40.8 us (2.4 TB/s). There two CTAs an SM take 34,000 cycles a wave: 11,000
-// to load, 4000 to sum, 3000 to exchange, 14,000 to normalise and store (8000
+// one launch 8.6 to 10 us (2.5 TB/s: one wave of CTAs that load, sum, meet and store in
+// turn, 14,000 cycles), 64 windows 45.9 us (4.3 TB/s); 64 x 375 x 1024 bf16 in one
+// group 37.3 us (2.6 TB/s). There two CTAs an SM took 34,000 cycles a wave when it was
+// 39.6 us: 11,000 to load, 4000 to sum, 3000 to exchange, 14,000 to normalise and store (8000
 // without SiLU: the special-function unit). 13 ragged windows of 7969 x 1000 fp16
-// in two launches 22 us. Quantised, 8 x 375 x 1024: 19 us, of which the second launch 8.
+// in two launches 23.5 us. Quantised, 8 x 375 x 1024: 18 us, of which the second launch 8.
+// With SiLU of values below -43 (weights of 60, say) those rows are normalised twice: 46 -> 66 us.
 #pragma once
 
 #include "pq8_rows.cuh"

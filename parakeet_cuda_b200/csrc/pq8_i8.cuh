@@ -212,9 +212,9 @@ __global__ void __launch_bounds__(kI8GemvThreads, 2) i8_gemv_kernel(const I8Para
 // Two accumulators let the next tile's products run under a tile's epilogue.
 //
 // Measured: 8192^3 350 us (3.14e15 operations/s, 0.93 of the rate taken for 8 bits:
-// twice the bf16 product's); 24,000 x 1024 x 4096 with SiLU to bf16 97.5 us (2.07e15;
-// the chip is at its power limit there, 990 W at 1.5 GHz, and the products
-// alone take 66); 3000 x 4096 x 1024 17.6 us (one wave and a bit of pairs);
+// twice the bf16 product's); 24,000 x 1024 x 4096 with SiLU to bf16 101 us (2.0e15;
+// the chip is at its power limit there, 990 W at 1.5 to 1.65 GHz, and the products
+// alone take 66); 3000 x 4096 x 1024 15.3 to 17.6 us (64 pair tiles on 74 pairs);
 // 375 x 1024 x 2048 GLU 5.6 us (3 us of launch, set-up and first loads).
 //
 // Warps: 0 and 2 TMA producers, 1 MMA issuer (and tensor-memory owner), 3
