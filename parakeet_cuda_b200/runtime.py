@@ -388,6 +388,8 @@ class Runtime:
         quantised to 8 bits with one scale per output channel."""
         if isinstance(w, tuple):
             raw, n, k = w
+            if k % 32:
+                raise ValueError(f'a Q8_0 row is whole blocks of 32, got {k} columns')
             blocks = _host_bytes(raw).to(self.device)
             if blocks.numel() != n * k // 32 * 34:
                 raise ValueError(f'expected {n * k // 32 * 34} Q8_0 bytes for [{n}, {k}], got {blocks.numel()}')

@@ -511,3 +511,12 @@ def test_int8_rows_whose_memory_leaves_the_device(rt):
         assert torch.equal(rt.linear_i8(rows, w8), want)
     with pytest.raises(ValueError):
         rt.linear_i8(x.cpu(), w8)
+
+
+def test_int8_weight_refuses_partial_blocks(rt):
+    """Q8_0 rows that are not whole blocks: two rows of 16 are no block of 32."""
+    blocks = q8_0_blocks(np.random.default_rng(1), 3, 32)
+    assert rt.int8_weight((blocks, 3, 32)).k == 32
+    for count, n, k in ((2, 4, 16), (3, 2, 48), (1, 2, 16), (2, 3, 32)):  # (the last: too few bytes)
+        with pytest.raises(ValueError):
+            rt.int8_weight((blocks[:count], n, k))
